@@ -5,7 +5,8 @@
  * allocates or frees.  Work is enqueued on `stream` and the call returns
  * without synchronising.  Return value: SSD_OK (0) or a negative SSD_ERR_*
  * code, in which case nothing was launched (ssd_forward_static, which runs
- * four stages, says below what holds for it).  All tensors are contiguous fp32.
+ * four stages, says below what holds for it).  All tensors are contiguous fp32
+ * unless an entry point says otherwise.
  *
  * Citations name the file of the So-cean/mamba-ascendc tree whose interface
  * the entry point stands in for.
@@ -291,6 +292,84 @@ int ssd_block_conv_split_fwd(const float* xbc, long long row_stride, const float
 int ssd_block_conv_silu_fwd(const float* xbc, long long row_stride, const float* weight, const float* bias,
                             float* x_out, float* b_out, float* c_out, int batch, int seqlen, int d_in, int gn,
                             ssd_stream_t stream);
+
+/* ---------------------------------------------------------------- operators around a selective state space layer
+ *
+ * Activations are fp32, bf16 or fp16 (`dtype`), parameters fp32 or, where a record has a flag for it, the activations' type.
+ * Rows have their columns side by side; distances between rows are given in elements (`*_stride`), so that column slices of
+ * a wider matrix are read where they lie.  Outputs are contiguous.  Sums, states and norms are held in fp32.
+ *
+ * Sequences: a batch [rows, tokens, ...] (cu_seqlens null), or packed one behind another in [tokens, ...] with sequence s from
+ * cu_seqlens[s] (0 for s = 0) to cu_seqlens[s + 1]; entries out of range are cut off at the tokens.  Outputs of tokens
+ * behind the last sequence are zeros. */
+enum { SSD_F32 = 0, SSD_BF16 = 1, SSD_F16 = 2 };
+
+/* Root-mean-square norm with the residual's addition: stream = x + residual; out = stream * rstd * weight with
+ * rstd = (mean(stream^2) + eps)^-1/2, of the sum before it is rounded to the residual's type.
+ * `out` (null with q): the activations' type.  `q`: e4m3 values of out / scale instead, with scale per `group` columns (a power of two from
+ * 32 to 128 that divides width; 0: per row), largest magnitude / 448 or 1 where that is 0, written to scales [rows, width / group];
+ * or, where `static_scale` is not null, that one scale.  width up to 16384. */
+typedef struct SsdNormArgs {
+    const void *x, *residual, *weight, *static_scale;
+    void *out, *stream, *q; /* stream: x + residual in the residual's type, null without a residual */
+    float *scales, *rstd;   /* rstd [rows], null = not wanted */
+    int64_t rows, x_stride, residual_stride;
+    int32_t width, dtype, residual_f32, weight_f32, group;
+    float eps;
+} SsdNormArgs;
+int ssd_rms_norm_fwd(const SsdNormArgs* args, ssd_stream_t stream);
+
+/* Its gradients: dx (and the same in the residual's type, dresidual: null = not wanted) and dweight (null = not wanted) from dout
+ * and dstream (null = zeros).  The sum that was normed is stream + addend: `stream` in the residual's type is the residual and
+ * `addend` is x; or stream is x + residual, or x where there was no residual, and addend is null.  rstd is the forward call's.
+ * `work`: ssd_rms_norm_work_bytes(). */
+typedef struct SsdNormGradArgs {
+    const void *dout, *dstream, *stream, *addend, *weight;
+    const float* rstd;
+    void *dx, *dresidual, *dweight;
+    float* work;
+    int64_t rows, dout_stride, dstream_stride, stream_stride, addend_stride;
+    int32_t width, dtype, residual_f32, weight_f32;
+} SsdNormGradArgs;
+size_t ssd_rms_norm_work_bytes(int64_t rows, int width, int dtype);
+int ssd_rms_norm_bwd(const SsdNormGradArgs* args, ssd_stream_t stream);
+
+/* Depthwise causal convolution of width 2 to 4 along the tokens: pre[t,c] = bias[c] + sum_k weight[c,k] in[t - (width-1) + k, c] and
+ * out = silu(pre) or pre, where in[-1], in[-2], ... are the last rows of initial_state [rows, width - 1, channels] (null = zeros).
+ * final_state (null = not wanted): the last width - 1 inputs of each sequence, those of its initial state among them where
+ * it is shorter. */
+typedef struct SsdConvArgs {
+    const void *x, *weight, *bias, *initial_state;
+    const int32_t* cu_seqlens;
+    void *out, *final_state;
+    int64_t tokens, batch_stride, token_stride; /* of x */
+    int32_t rows, channels, width, dtype, weight_f32, silu;
+} SsdConvArgs;
+int ssd_short_conv_fwd(const SsdConvArgs* args, ssd_stream_t stream);
+
+/* Its gradients from dout (contiguous) and dfinal (null = zeros): dx (contiguous), dinitial, dweight, dbias (each null = not
+ * wanted; dweight and dbias together).  `forward` as in the forward call, its outputs aside.  `work`: ssd_short_conv_work_bytes(). */
+typedef struct SsdConvGradArgs {
+    SsdConvArgs forward;
+    const void *dout, *dfinal;
+    void *dx, *dinitial, *dweight, *dbias;
+    float* work;
+} SsdConvGradArgs;
+size_t ssd_short_conv_work_bytes(const SsdConvArgs* args);
+int ssd_short_conv_bwd(const SsdConvGradArgs* args, ssd_stream_t stream);
+
+/* One token of each of `rows` sequences: x [rows, channels] with rows x_stride apart, states [slots, width - 1, channels] with slots
+ * state_stride (state_out_stride) apart.  Row r takes slot slots[r] (r itself where slots is null): its state is read from
+ * `state`, and the one with the token is written to `state_out`, which may be `state`.  A slot below zero or behind the last is none: the row's
+ * output is zeros.  A slot that several rows name takes them one after another, in their order. */
+typedef struct SsdConvStepArgs {
+    const void *x, *weight, *bias, *state;
+    const int32_t* slots;
+    void *state_out, *out;
+    int64_t x_stride, state_stride, state_out_stride;
+    int32_t rows, slot_count, channels, width, dtype, weight_f32, silu;
+} SsdConvStepArgs;
+int ssd_short_conv_step(const SsdConvStepArgs* args, ssd_stream_t stream);
 
 /* ---------------------------------------------------------------- forward without any allocation
  *

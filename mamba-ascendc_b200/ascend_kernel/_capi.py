@@ -50,6 +50,29 @@ SsdForwardArgs = _args("SsdForwardArgs", "x dt dt_bias A bm cm D z initial_state
 SsdBackwardArgs = _args("SsdBackwardArgs", "x dt dt_bias A bm cm D z y dout dfinal forward_work dx ddt dA dB dC dD dz "
                                            "d_dt_bias d_initial work status")
 
+SSD_F32, SSD_BF16, SSD_F16 = 0, 1, 2
+
+
+def _record(name: str, *groups):
+    """Mirror of an argument record that is laid out as groups of (type, names)."""
+    fields = [(f, kind) for kind, names in groups for f in names.split()]
+    return type(name, (ctypes.Structure,), {"_fields_": fields})
+
+
+_P, _I64, _I32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+SsdNormArgs = _record("SsdNormArgs", (_P, "x residual weight static_scale out stream q scales rstd"),
+                      (_I64, "rows x_stride residual_stride"), (_I32, "width dtype residual_f32 weight_f32 group"),
+                      (ctypes.c_float, "eps"))
+SsdNormGradArgs = _record("SsdNormGradArgs", (_P, "dout dstream stream addend weight rstd dx dresidual dweight work"),
+                          (_I64, "rows dout_stride dstream_stride stream_stride addend_stride"),
+                          (_I32, "width dtype residual_f32 weight_f32"))
+SsdConvArgs = _record("SsdConvArgs", (_P, "x weight bias initial_state cu_seqlens out final_state"),
+                      (_I64, "tokens batch_stride token_stride"), (_I32, "rows channels width dtype weight_f32 silu"))
+SsdConvGradArgs = _record("SsdConvGradArgs", (SsdConvArgs, "forward"), (_P, "dout dfinal dx dinitial dweight dbias work"))
+SsdConvStepArgs = _record("SsdConvStepArgs", (_P, "x weight bias state slots state_out out"),
+                          (_I64, "x_stride state_stride state_out_stride"),
+                          (_I32, "rows slot_count channels width dtype weight_f32 silu"))
+
 
 def library_path() -> Path:
     override = os.environ.get("SSD_B200_LIBRARY")
@@ -112,6 +135,13 @@ SIGNATURES = {
     "ssd_linear_work_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int]),
     "ssd_linear_pays": (ctypes.c_int, [ctypes.c_longlong, ctypes.c_int, ctypes.c_int]),
     "ssd_linear_fwd": (ctypes.c_int, [_p, _p, _p, _p, ctypes.c_longlong, ctypes.c_int, ctypes.c_int, _p, _p, _p]),
+    "ssd_rms_norm_fwd": (ctypes.c_int, [ctypes.POINTER(SsdNormArgs), _p]),
+    "ssd_rms_norm_work_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int, ctypes.c_int]),
+    "ssd_rms_norm_bwd": (ctypes.c_int, [ctypes.POINTER(SsdNormGradArgs), _p]),
+    "ssd_short_conv_fwd": (ctypes.c_int, [ctypes.POINTER(SsdConvArgs), _p]),
+    "ssd_short_conv_work_bytes": (ctypes.c_size_t, [ctypes.POINTER(SsdConvArgs)]),
+    "ssd_short_conv_bwd": (ctypes.c_int, [ctypes.POINTER(SsdConvGradArgs), _p]),
+    "ssd_short_conv_step": (ctypes.c_int, [ctypes.POINTER(SsdConvStepArgs), _p]),
     "ssd_use_state_scan": (ctypes.c_int, [_shape_p, ctypes.c_int]),
     "ssd_forward_work_bytes": (ctypes.c_size_t, [_shape_p]),
     "ssd_backward_work_bytes": (ctypes.c_size_t, [_shape_p, ctypes.c_int, ctypes.c_int]),

@@ -1,0 +1,374 @@
+// Root-mean-square norm with the residual's addition, its gradients, and the same norm with an output in 8 bits:
+//
+//   v = x + residual ;  r = (mean(v^2) + eps)^-1/2 ;  out = v r w              q = e4m3(out / s), s = max|out| / 448 per row or group
+//   g = dout w ;  dv = r (g - v r mean(g v r)) + dstream ;  dw = sum_rows dout v r
+//
+// What bounds them: HBM.  Each element is loaded once, held in registers as fp32 between the row's sum and the output, and
+// stored once.  A thread owns vectors of 16 bytes (`VEC` elements), ITER of them, `tpr` threads make a row: rows of up to 4
+// vectors per lane are a warp's, longer ones a CTA's.  Scalar loads take the same elements where rows are not aligned.
+#include <cuda_fp8.h>
+
+#include "ssd_vec.cuh"
+
+namespace ssd {
+
+namespace {
+
+constexpr int kNormMaxWidth = 16384;
+constexpr int kNormThreads = 512;
+
+template <class T>
+constexpr int kNormVec = 16 / static_cast<int>(sizeof(T));
+
+// Sums and maxima over the tpr threads of a row; `part` has room for 2 x 32 floats per call site.
+struct Reduced {
+    float sum, top;
+};
+template <bool TOP>
+__device__ __forceinline__ Reduced reduce_row(float sum, float top, int tpr, float* part) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (TOP) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    if (tpr > 32) {  // then the row is the whole CTA's
+        const int warp = threadIdx.x >> 5, warps = tpr >> 5;
+        if ((threadIdx.x & 31) == 0) {
+            part[warp] = sum;
+            if (TOP) part[32 + warp] = top;
+        }
+        __syncthreads();
+        sum = 0.f;
+        for (int i = 0; i < warps; ++i) {
+            sum += part[i];
+            if (TOP) top = max_nan(top, part[32 + i]);
+        }
+    }
+    return {sum, top};
+}
+
+template <class T, class R, int ITER, bool VECTOR, bool QUANT>
+__global__ void __launch_bounds__(kNormThreads)
+norm_fwd_kernel(const SsdNormArgs a, int tpr) {
+    constexpr int VEC = kNormVec<T>;
+    __shared__ float part[64];
+    const int at = threadIdx.x % tpr;
+    const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
+    const bool live = row < a.rows;
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const R* res = static_cast<const R*>(a.residual) + row * a.residual_stride;
+    float v[ITER][VEC], w[ITER][VEC];
+    float r[ITER][VEC];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int c = (at + i * tpr) * VEC, n = live ? min(a.width - c, VEC) : 0;
+        load_f<VECTOR>(v[i], x + c, n);
+        if (a.residual != nullptr) load_f<VECTOR>(r[i], res + c, n);
+    }
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int c = (at + i * tpr) * VEC, n = min(a.width - c, VEC);
+        if (a.weight_f32)
+            load_f<VECTOR>(w[i], static_cast<const float*>(a.weight) + c, n);
+        else
+            load_f<VECTOR>(w[i], static_cast<const T*>(a.weight) + c, n);
+    }
+    float sum = 0.f, top = 0.f;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int c = (at + i * tpr) * VEC, n = live ? min(a.width - c, VEC) : 0;
+        if (a.residual != nullptr) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[i][j] += r[i][j];
+            store_f<VECTOR>(static_cast<R*>(a.stream) + row * a.width + c, v[i], n);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            sum = fmaf(v[i][j], v[i][j], sum);
+            if (QUANT) top = max_nan(top, fabsf(v[i][j] * w[i][j]));
+        }
+    }
+    const bool row_scale = QUANT && a.static_scale == nullptr && a.group == 0;
+    const Reduced red = QUANT ? reduce_row<true>(sum, top, tpr, part) : reduce_row<false>(sum, 0.f, tpr, part);
+    const float rstd = rsqrtf(red.sum / static_cast<float>(a.width) + a.eps);
+    if (a.rstd != nullptr && live && at == 0) a.rstd[row] = rstd;
+    if constexpr (!QUANT) {
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int c = (at + i * tpr) * VEC, n = live ? min(a.width - c, VEC) : 0;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[i][j] = v[i][j] * rstd * w[i][j];
+            store_f<VECTOR>(static_cast<T*>(a.out) + row * a.width + c, v[i], n);
+        }
+    } else {
+        float scale = 1.f;
+        if (a.static_scale != nullptr) scale = *static_cast<const float*>(a.static_scale);
+        if (row_scale) {
+            // rstd is positive, so the largest |v w| is the largest |out| but for rstd
+            scale = red.top * rstd / 448.f;
+            if (scale == 0.f) scale = 1.f;
+            if (live && at == 0) a.scales[row] = scale;
+        }
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int c = (at + i * tpr) * VEC, n = live ? min(a.width - c, VEC) : 0;
+            float y[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) y[j] = v[i][j] * rstd * w[i][j];
+            if (a.group != 0 && a.static_scale == nullptr) {
+                // a group is group / VEC neighbouring lanes, a power of two that divides 32
+                float m = 0.f;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) m = max_nan(m, fabsf(y[j]));
+                for (int o = a.group / VEC / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                scale = m / 448.f;
+                if (scale == 0.f) scale = 1.f;
+                if (n > 0 && c % a.group == 0) a.scales[row * (a.width / a.group) + c / a.group] = scale;
+            }
+            // a reciprocal, but for scales so small that it would overflow
+            const bool tiny = fabsf(scale) < 1e-30f;
+            const float inv = tiny ? 1.f : 1.f / scale;
+            alignas(8) unsigned char q[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; j += 2) {
+                const float2 t = tiny ? make_float2(y[j] / scale, y[j + 1] / scale) : make_float2(y[j] * inv, y[j + 1] * inv);
+                *reinterpret_cast<unsigned short*>(q + j) = __nv_cvt_float2_to_fp8x2(t, __NV_SATFINITE, __NV_E4M3);
+            }
+            unsigned char* dst = static_cast<unsigned char*>(a.q) + row * a.width + c;
+            if constexpr (VECTOR) {
+                using B = typename Bits<VEC>::type;
+                if (n > 0) *reinterpret_cast<B*>(dst) = *reinterpret_cast<B*>(q);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (j < n) dst[j] = q[j];
+            }
+        }
+    }
+}
+
+// CTAs walk the rows at a distance of the grid, so that a thread keeps its columns and sums their share of dw in registers;
+// the CTA's rows are added up in shared memory and leave as one row of `work`, which norm_dw_kernel sums in a fixed order.
+template <class T, class R, int ITER, bool VECTOR>
+__global__ void __launch_bounds__(kNormThreads)
+norm_bwd_kernel(const SsdNormGradArgs a, int tpr) {
+    constexpr int VEC = kNormVec<T>;
+    __shared__ float part[2][64];
+    extern __shared__ float norm_rows[];  // [rows of the CTA][width], only where there are several
+    const int at = threadIdx.x % tpr, rows_here = blockDim.x / tpr, mine = threadIdx.x / tpr;
+    float w[ITER][VEC], dw[ITER][VEC];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int c = (at + i * tpr) * VEC, n = min(a.width - c, VEC);
+        if (a.weight_f32)
+            load_f<VECTOR>(w[i], static_cast<const float*>(a.weight) + c, n);
+        else
+            load_f<VECTOR>(w[i], static_cast<const T*>(a.weight) + c, n);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) dw[i][j] = 0.f;
+    }
+    int parity = 0;
+    for (long long first = static_cast<long long>(blockIdx.x) * rows_here; first < a.rows;
+         first += static_cast<long long>(gridDim.x) * rows_here) {
+        const long long row = first + mine;
+        const bool live = row < a.rows;
+        const float rstd = live ? a.rstd[row] : 0.f;
+        float v[ITER][VEC], g[ITER][VEC], s[ITER][VEC];
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int c = (at + i * tpr) * VEC, n = live ? min(a.width - c, VEC) : 0;
+            load_f<VECTOR>(v[i], static_cast<const R*>(a.stream) + row * a.stream_stride + c, n);
+            load_f<VECTOR>(g[i], static_cast<const T*>(a.dout) + row * a.dout_stride + c, n);
+            if (a.dstream != nullptr)
+                load_f<VECTOR>(s[i], static_cast<const R*>(a.dstream) + row * a.dstream_stride + c, n);
+            if (a.addend != nullptr) {
+                float u[VEC];
+                load_f<VECTOR>(u, static_cast<const T*>(a.addend) + row * a.addend_stride + c, n);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[i][j] += u[j];
+            }
+        }
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                v[i][j] *= rstd;
+                dw[i][j] = fmaf(g[i][j], v[i][j], dw[i][j]);
+                g[i][j] *= w[i][j];
+                dot = fmaf(g[i][j], v[i][j], dot);
+            }
+        }
+        const float mean = reduce_row<false>(dot, 0.f, tpr, part[parity]).sum / static_cast<float>(a.width);
+        parity ^= 1;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int c = (at + i * tpr) * VEC, n = live ? min(a.width - c, VEC) : 0;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                g[i][j] = rstd * fmaf(-v[i][j], mean, g[i][j]);
+                if (a.dstream != nullptr) g[i][j] += s[i][j];
+            }
+            store_f<VECTOR>(static_cast<T*>(a.dx) + row * a.width + c, g[i], n);
+            if (a.dresidual != nullptr) store_f<VECTOR>(static_cast<R*>(a.dresidual) + row * a.width + c, g[i], n);
+        }
+    }
+    if (a.dweight == nullptr) return;
+    float* table = a.work + static_cast<long long>(blockIdx.x) * a.width;
+    if (rows_here > 1) {
+#pragma unroll
+        for (int i = 0; i < ITER; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const int c = (at + i * tpr) * VEC + j;
+                if (c < a.width) norm_rows[mine * a.width + c] = dw[i][j];
+            }
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
+            float sum = 0.f;
+            for (int k = 0; k < rows_here; ++k) sum += norm_rows[k * a.width + c];
+            table[c] = sum;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int c = (at + i * tpr) * VEC;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (c + j < a.width) table[c + j] = dw[i][j];
+        }
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kSumCols * kSumRows)
+norm_dw_kernel(const float* table, long long rows, int width, void* dweight, int f32) {
+    column_sums(table, rows, width, [&](long long c, float v) { store_param<T>(dweight, f32, c, v); });
+}
+
+struct NormGeometry {
+    int tpr, iter, rows_here;
+};
+// Threads per row and vectors per thread.  Rows of up to 128 vectors are a warp's; of longer ones a thread takes one vector where
+// there are few rows (latency counts) and up to `most` where they fill the GPU anyway (fewer threads to reduce over).
+NormGeometry norm_geometry(long long rows, int width, int vec, int most) {
+    const int vecs = (width + vec - 1) / vec;
+    const bool many = rows >= 8LL * sm_count();
+    NormGeometry g{32, 1, 1};
+    if (vecs <= 32 * most && (many || vecs <= 32)) {
+        g.iter = vecs <= 32 ? 1 : vecs <= 64 ? 2 : 4;
+    } else {
+        int iter = many ? most : 1;
+        while ((vecs + iter - 1) / iter > kNormThreads) iter *= 2;
+        g.iter = iter;
+        g.tpr = ((vecs + iter - 1) / iter + 31) / 32 * 32;
+    }
+    g.rows_here = g.tpr == 32 && many ? 8 : 1;
+    return g;
+}
+constexpr int kNormGradIter = 2;
+unsigned norm_bwd_grid(long long rows, const NormGeometry& g) {
+    const long long all = (rows + g.rows_here - 1) / g.rows_here;
+    const long long resident = static_cast<long long>(sm_count()) * (1024 / (g.tpr * g.rows_here));
+    return static_cast<unsigned>(all < resident ? all : resident);
+}
+
+template <class T, class F>
+int with_residual_type(int residual_f32, F f) {
+    if constexpr (sizeof(T) == 4) {
+        return f(T{});
+    } else {
+        return residual_f32 ? f(float{}) : f(T{});
+    }
+}
+template <class T, class F>
+int with_iter(int iter, F f) {
+    switch (iter) {
+        case 1: return f(std::integral_constant<int, 1>{});
+        case 2: return f(std::integral_constant<int, 2>{});
+        case 4: return f(std::integral_constant<int, 4>{});
+        default: return f(std::integral_constant<int, kNormMaxWidth / kNormThreads / kNormVec<T>>{});
+    }
+}
+
+}  // namespace
+
+}  // namespace ssd
+
+extern "C" int ssd_rms_norm_fwd(const SsdNormArgs* args, ssd_stream_t stream) {
+    using namespace ssd;
+    if (args == nullptr) return SSD_ERR_NULL;
+    const SsdNormArgs& a = *args;
+    if (a.rows <= 0 || a.width <= 0 || a.x_stride < 0 || a.residual_stride < 0) return SSD_ERR_SHAPE;
+    if (a.width > kNormMaxWidth) return SSD_ERR_UNSUPPORTED;
+    const bool quant = a.q != nullptr;
+    if (!a.x || !a.weight || (!quant && !a.out) || (a.residual && !a.stream) || (quant && !a.static_scale && !a.scales))
+        return SSD_ERR_NULL;
+    if (a.group != 0 && ((a.group != 32 && a.group != 64 && a.group != 128) || a.width % a.group != 0)) return SSD_ERR_SHAPE;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return with_type(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        return with_residual_type<T>(a.residual_f32, [&](auto r) {
+            using R = decltype(r);
+            const int vec = kNormVec<T>;
+            const NormGeometry g = norm_geometry(a.rows, a.width, vec, 4);
+            const long long blocks = (a.rows + g.rows_here - 1) / g.rows_here;
+            if (blocks > 0x7fffffffLL) return static_cast<int>(SSD_ERR_RANGE);
+            const bool vector = aligned16(a.x, a.residual, a.weight, a.out, a.stream, a.q) && multiple_of(a.width, vec) &&
+                                multiple_of(a.x_stride, vec) && multiple_of(a.residual_stride, vec);
+            return with_iter<T>(g.iter, [&](auto it) {
+                constexpr int I = decltype(it)::value;
+                const auto launch = [&](auto kernel) {
+                    launch_plain(kernel, static_cast<unsigned>(blocks), g.tpr * g.rows_here, 0, st, a, g.tpr);
+                };
+                if (quant)
+                    vector ? launch(norm_fwd_kernel<T, R, I, true, true>) : launch(norm_fwd_kernel<T, R, I, false, true>);
+                else
+                    vector ? launch(norm_fwd_kernel<T, R, I, true, false>) : launch(norm_fwd_kernel<T, R, I, false, false>);
+                return launch_status();
+            });
+        });
+    });
+}
+
+extern "C" size_t ssd_rms_norm_work_bytes(int64_t rows, int width, int dtype) {
+    using namespace ssd;
+    if (rows <= 0 || width <= 0 || width > kNormMaxWidth || dtype < SSD_F32 || dtype > SSD_F16) return 0;
+    const NormGeometry g = norm_geometry(rows, width, dtype == SSD_F32 ? 4 : 8, kNormGradIter);
+    return sizeof(float) * static_cast<size_t>(norm_bwd_grid(rows, g)) * width;
+}
+
+extern "C" int ssd_rms_norm_bwd(const SsdNormGradArgs* args, ssd_stream_t stream) {
+    using namespace ssd;
+    if (args == nullptr) return SSD_ERR_NULL;
+    const SsdNormGradArgs& a = *args;
+    if (a.rows <= 0 || a.width <= 0 || a.dout_stride < 0 || a.dstream_stride < 0 || a.stream_stride < 0 ||
+        a.addend_stride < 0) return SSD_ERR_SHAPE;
+    if (a.width > kNormMaxWidth) return SSD_ERR_UNSUPPORTED;
+    if (!a.dout || !a.stream || !a.weight || !a.rstd || !a.dx || (a.dweight && !a.work)) return SSD_ERR_NULL;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return with_type(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        return with_residual_type<T>(a.residual_f32, [&](auto r) {
+            using R = decltype(r);
+            const int vec = kNormVec<T>;
+            const NormGeometry g = norm_geometry(a.rows, a.width, vec, kNormGradIter);
+            const unsigned grid = norm_bwd_grid(a.rows, g);
+            const size_t smem = g.rows_here > 1 ? sizeof(float) * g.rows_here * a.width : 0;
+            const bool vector = aligned16(a.dout, a.dstream, a.stream, a.addend, a.weight, a.dx, a.dresidual) &&
+                                multiple_of(a.width, vec) && multiple_of(a.dout_stride, vec) &&
+                                multiple_of(a.dstream_stride, vec) && multiple_of(a.stream_stride, vec) &&
+                                multiple_of(a.addend_stride, vec);
+            const int rc = with_iter<T>(g.iter, [&](auto it) {
+                constexpr int I = decltype(it)::value;
+                const auto launch = [&](auto kernel) { launch_plain(kernel, grid, g.tpr * g.rows_here, smem, st, a, g.tpr); };
+                vector ? launch(norm_bwd_kernel<T, R, I, true>) : launch(norm_bwd_kernel<T, R, I, false>);
+                return launch_status();
+            });
+            if (rc != SSD_OK || a.dweight == nullptr) return rc;
+            launch_plain(norm_dw_kernel<T>, static_cast<unsigned>((a.width + kSumCols - 1) / kSumCols), kSumCols * kSumRows, 0, st,
+                         a.work, static_cast<long long>(grid), a.width, a.dweight, a.weight_f32);
+            return launch_status();
+        });
+    });
+}

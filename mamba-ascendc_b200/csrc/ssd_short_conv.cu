@@ -1,0 +1,414 @@
+// Short causal convolution along the tokens, one filter of 2 to 4 taps per channel, for batches and packed sequences, its
+// gradients, and the step of one token:
+//
+//   pre[t] = bias + sum_k w[k] in[t - (W-1) + k] ;  out = pre sigmoid(pre) or pre
+//   dpre = dout silu'(pre) ;  din[t] = sum_k w[k] dpre[t + (W-1) - k] ;  dw[k] = sum_t dpre[t] in[t - (W-1) + k]
+//
+// What bounds it: HBM.  A thread owns V neighbouring channels and walks an item of consecutive tokens with the last W
+// inputs in registers, the loads of kAhead tokens in flight; lanes lie along the channels.  An item reads W-1 tokens of
+// the one before it again (out of L2).
+#include "ssd_vec.cuh"
+
+namespace ssd {
+
+namespace {
+
+constexpr int kConvThreads = 128;
+constexpr int kConvAhead = 8;
+
+struct ConvDims {
+    SeqMap map;
+    int channel_blocks;
+};
+
+template <class T, int V, int W>
+struct Filter {
+    float w[W][V], bias[V];
+    __device__ __forceinline__ void load(const SsdConvArgs& a, int c) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const bool in = c + j < a.channels;
+#pragma unroll
+            for (int k = 0; k < W; ++k)
+                w[k][j] = in ? load_param<T>(a.weight, a.weight_f32, static_cast<long long>(c + j) * W + k) : 0.f;
+            bias[j] = in && a.bias != nullptr ? load_param<T>(a.bias, a.weight_f32, c + j) : 0.f;
+        }
+    }
+};
+
+// Input of the sequence at t in [-(W-1), len): of the initial state where t < 0.
+template <class T, int V, int W, bool VECTOR>
+__device__ __forceinline__ void load_input(float (&f)[V], const SsdConvArgs& a, const SeqMap& m, const Span& s, int t, int c,
+                                           int n) {
+    if (t >= 0) {
+        load_f<VECTOR>(f, static_cast<const T*>(a.x) + token_row(m, s, a.batch_stride, a.token_stride, t) + c, n);
+    } else if (a.initial_state != nullptr) {
+        load_f<VECTOR>(f, static_cast<const T*>(a.initial_state) +
+                              (static_cast<long long>(s.seq) * (W - 1) + (t + W - 1)) * a.channels + c, n);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = 0.f;
+    }
+}
+
+template <class T, int V, int W, bool VECTOR>
+__global__ void __launch_bounds__(kConvThreads)
+conv_fwd_kernel(const SsdConvArgs a, const ConvDims d) {
+    const long long item = blockIdx.x / d.channel_blocks;
+    const int c = (blockIdx.x % d.channel_blocks * kConvThreads + threadIdx.x) * V;
+    Span s;
+    if (!locate(d.map, item, s)) return;
+    const int n = min(a.channels - c, V);
+    if (n <= 0) return;
+    T* out = static_cast<T*>(a.out) + ((d.map.cu == nullptr ? s.seq * d.map.tokens : 0) + s.origin) * a.channels + c;
+    if (s.pad) {
+        const float zero[V] = {};
+        for (int t = s.t0; t < s.t1; ++t) store_f<VECTOR>(out + static_cast<long long>(t) * a.channels, zero, n);
+        return;
+    }
+    Filter<T, V, W> f;
+    f.load(a, c);
+    float held[W][V];  // the last W inputs, held[W-1] the newest
+#pragma unroll
+    for (int k = 1; k < W; ++k) load_input<T, V, W, VECTOR>(held[k], a, d.map, s, s.t0 - W + k, c, n);
+    const T* x = static_cast<const T*>(a.x) + token_row(d.map, s, a.batch_stride, a.token_stride, 0) + c;
+    for (int t = s.t0; t < s.t1; t += kConvAhead) {
+        float next[kConvAhead][V];
+#pragma unroll
+        for (int i = 0; i < kConvAhead; ++i) load_f<VECTOR>(next[i], x + (t + i) * a.token_stride, t + i < s.t1 ? n : 0);
+#pragma unroll
+        for (int i = 0; i < kConvAhead; ++i) {
+            float o[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+#pragma unroll
+                for (int k = 0; k + 1 < W; ++k) held[k][j] = held[k + 1][j];
+                held[W - 1][j] = next[i][j];
+                float p = f.bias[j];
+#pragma unroll
+                for (int k = 0; k < W; ++k) p = fmaf(f.w[k][j], held[k][j], p);
+                o[j] = a.silu ? p * sigmoid_fast(p) : p;
+            }
+            if (t + i < s.t1) store_f<VECTOR>(out + static_cast<long long>(t + i) * a.channels, o, n);
+        }
+    }
+    if (s.last && a.final_state != nullptr) {
+        T* fin = static_cast<T*>(a.final_state) + static_cast<long long>(s.seq) * (W - 1) * a.channels + c;
+#pragma unroll
+        for (int k = 0; k + 1 < W; ++k) {
+            float v[V];
+            load_input<T, V, W, VECTOR>(v, a, d.map, s, s.len - (W - 1) + k, c, n);
+            store_f<VECTOR>(fin + static_cast<long long>(k) * a.channels, v, n);
+        }
+    }
+}
+
+// Items are dealt to the CTAs of a channel block at a distance, so that a thread keeps its channels and sums their share of
+// dw in registers; each CTA leaves one row of `work` [CTAs][W + 1][channels], which conv_dw_kernel sums in a fixed order.
+// At token t the thread has dpre[t - (W-1) .. t], which is what the gradient of input t - (W-1) takes; the item's last
+// W-1 inputs take W-1 tokens of the next one, and the first item's walk starts W-1 inputs early, in the initial state.
+template <class T, int V, int W, bool VECTOR>
+__global__ void __launch_bounds__(kConvThreads)
+conv_bwd_kernel(const SsdConvGradArgs g, const ConvDims d, int slices) {
+    const SsdConvArgs& a = g.forward;
+    const int slice = blockIdx.x / d.channel_blocks;
+    const int c = (blockIdx.x % d.channel_blocks * kConvThreads + threadIdx.x) * V;
+    const int n = max(min(a.channels - c, V), 0);
+    Filter<T, V, W> f;
+    f.load(a, c);
+    float dw[W][V], db[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        db[j] = 0.f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) dw[k][j] = 0.f;
+    }
+    const long long items = d.map.items();
+    for (long long item = slice; item < items; item += slices) {
+        Span s;
+        if (!locate(d.map, item, s) || n == 0) continue;
+        const long long first_row = (d.map.cu == nullptr ? s.seq * d.map.tokens : 0) + s.origin;
+        T* dx = static_cast<T*>(g.dx) + first_row * a.channels + c;
+        const T* dout = static_cast<const T*>(g.dout) + first_row * a.channels + c;
+        if (s.pad) {
+            const float zero[V] = {};
+            for (int t = s.t0; t < s.t1; ++t) store_f<VECTOR>(dx + static_cast<long long>(t) * a.channels, zero, n);
+            continue;
+        }
+        const T* x = static_cast<const T*>(a.x) + token_row(d.map, s, a.batch_stride, a.token_stride, 0) + c;
+        float held[W][V], dpre[W][V];
+#pragma unroll
+        for (int k = 1; k < W; ++k) {
+            load_input<T, V, W, VECTOR>(held[k], a, d.map, s, s.t0 - W + k, c, n);
+#pragma unroll
+            for (int j = 0; j < V; ++j) dpre[k][j] = 0.f;
+        }
+        constexpr int kAhead = kConvAhead / 2;
+        for (int t = s.t0; t < s.t1 + W - 1; t += kAhead) {
+            float xs[kAhead][V], ds[kAhead][V];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int in = t + i < s.len && t + i < s.t1 + W - 1 ? n : 0;
+                load_f<VECTOR>(xs[i], x + (t + i) * a.token_stride, in);
+                load_f<VECTOR>(ds[i], dout + static_cast<long long>(t + i) * a.channels, in);
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int to = t + i - (W - 1);  // the input whose gradient is complete with this token
+                const bool mine = t + i < s.t1;
+                float o[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+#pragma unroll
+                    for (int k = 0; k + 1 < W; ++k) held[k][j] = held[k + 1][j], dpre[k][j] = dpre[k + 1][j];
+                    held[W - 1][j] = xs[i][j];
+                    float e = ds[i][j];
+                    if (a.silu) {
+                        float p = f.bias[j];
+#pragma unroll
+                        for (int k = 0; k < W; ++k) p = fmaf(f.w[k][j], held[k][j], p);
+                        const float gate = sigmoid_fast(p);
+                        // behind the sequence's end there is no gradient, and inputs that are not there may make 0 * inf
+                        e = e == 0.f ? 0.f : e * gate * fmaf(p, 1.f - gate, 1.f);
+                    }
+                    dpre[W - 1][j] = e;
+                    if (mine) {
+                        db[j] += e;
+#pragma unroll
+                        for (int k = 0; k < W; ++k) dw[k][j] = fmaf(e, held[k][j], dw[k][j]);
+                    }
+                    float sum = 0.f;
+#pragma unroll
+                    for (int k = 0; k < W; ++k) sum = fmaf(f.w[k][j], dpre[W - 1 - k][j], sum);
+                    o[j] = sum;
+                }
+                if (to >= s.t1 || (to < s.t0 && !s.first)) continue;
+                const int kept = to - (s.len - (W - 1));  // this input is row `kept` of the final state
+                if (kept >= 0 && g.dfinal != nullptr) {
+                    float df[V];
+                    load_f<VECTOR>(df, static_cast<const T*>(g.dfinal) +
+                                           (static_cast<long long>(s.seq) * (W - 1) + kept) * a.channels + c, n);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) o[j] += df[j];
+                }
+                if (to >= 0)
+                    store_f<VECTOR>(dx + static_cast<long long>(to) * a.channels, o, n);
+                else if (g.dinitial != nullptr)
+                    store_f<VECTOR>(static_cast<T*>(g.dinitial) +
+                                        (static_cast<long long>(s.seq) * (W - 1) + (to + W - 1)) * a.channels + c, o, n);
+            }
+        }
+    }
+    if (g.dweight == nullptr) return;
+    float* row = g.work + static_cast<long long>(slice) * (W + 1) * a.channels + c;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (j >= n) break;
+#pragma unroll
+        for (int k = 0; k < W; ++k) row[static_cast<long long>(k) * a.channels + j] = dw[k][j];
+        row[static_cast<long long>(W) * a.channels + j] = db[j];
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kSumCols * kSumRows)
+conv_dw_kernel(const float* table, long long rows, int channels, int width, void* dweight, void* dbias, int f32) {
+    column_sums(table, rows, static_cast<long long>(channels) * (width + 1), [&](long long col, float v) {
+        const long long k = col / channels, c = col - k * channels;
+        if (k < width)
+            store_param<T>(dweight, f32, c * width + k, v);
+        else if (dbias != nullptr)
+            store_param<T>(dbias, f32, c, v);
+    });
+}
+
+// A generation step: the state and the token in, the state moved on by one and the output out.  A thread owns V channels
+// of a row.  Rows that name the same slot are one another's successors: the first of them does the work of all, each
+// taking the inputs that the one before it left, so that nothing depends on the order of the CTAs.
+template <class T, int V, int W, bool VECTOR>
+__global__ void __launch_bounds__(kConvThreads)
+conv_step_kernel(const SsdConvStepArgs a, int channel_blocks) {
+    const int row = blockIdx.x / channel_blocks;
+    const int c = (blockIdx.x % channel_blocks * kConvThreads + threadIdx.x) * V;
+    const int n = min(a.channels - c, V);
+    long long slot = row;
+    bool shared = false;
+    if (a.slots != nullptr) {
+        slot = a.slots[row];
+        if (slot < 0 || slot >= a.slot_count) {
+            if (n > 0) {
+                const float zero[V] = {};
+                store_f<VECTOR>(static_cast<T*>(a.out) + static_cast<long long>(row) * a.channels + c, zero, n);
+            }
+            return;
+        }
+        bool before = false, after = false;
+        for (int r = threadIdx.x; r < a.rows; r += kConvThreads) {
+            const bool same = a.slots[r] == slot;
+            before |= same && r < row;
+            after |= same && r > row;
+        }
+        if (__syncthreads_or(before)) return;
+        shared = __syncthreads_or(after);
+    }
+    if (n <= 0) return;
+    const SsdConvArgs filter{nullptr, a.weight, a.bias, nullptr, nullptr, nullptr, nullptr, 0, 0, 0, 0, a.channels, W, a.dtype,
+                             a.weight_f32, a.silu};
+    float held[W][V];
+    const T* state = static_cast<const T*>(a.state) + slot * a.state_stride + c;
+#pragma unroll
+    for (int k = 1; k < W; ++k) load_f<VECTOR>(held[k], state + static_cast<long long>(k - 1) * a.channels, n);
+    Filter<T, V, W> f;
+    f.load(filter, c);
+    int r = row;
+    while (true) {
+        float x[V], o[V];
+        load_f<VECTOR>(x, static_cast<const T*>(a.x) + r * a.x_stride + c, n);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+#pragma unroll
+            for (int k = 0; k + 1 < W; ++k) held[k][j] = held[k + 1][j];
+            held[W - 1][j] = x[j];
+            float p = f.bias[j];
+#pragma unroll
+            for (int k = 0; k < W; ++k) p = fmaf(f.w[k][j], held[k][j], p);
+            o[j] = a.silu ? p * sigmoid_fast(p) : p;
+        }
+        store_f<VECTOR>(static_cast<T*>(a.out) + static_cast<long long>(r) * a.channels + c, o, n);
+        if (!shared) break;
+        do ++r;
+        while (r < a.rows && a.slots[r] != slot);
+        if (r >= a.rows) break;
+    }
+    T* next = static_cast<T*>(a.state_out) + slot * a.state_out_stride + c;
+#pragma unroll
+    for (int k = 1; k < W; ++k) store_f<VECTOR>(next + static_cast<long long>(k - 1) * a.channels, held[k], n);
+}
+
+int conv_check(const SsdConvArgs& a) {
+    if (a.rows <= 0 || a.tokens < 0 || (a.tokens == 0 && a.cu_seqlens == nullptr) || a.channels <= 0 || a.batch_stride < 0 ||
+        a.token_stride < 0)
+        return SSD_ERR_SHAPE;
+    if (a.width < 2 || a.width > 4) return SSD_ERR_UNSUPPORTED;
+    if (a.tokens > 0x7fffffff - (1 << 20) || a.rows > 0x7ffffff0) return SSD_ERR_RANGE;
+    if ((a.tokens > 0 && !a.x) || !a.weight) return SSD_ERR_NULL;
+    return SSD_OK;
+}
+template <class F>
+int with_width(int width, F f) {
+    switch (width) {
+        case 2: return f(std::integral_constant<int, 2>{});
+        case 3: return f(std::integral_constant<int, 3>{});
+        default: return f(std::integral_constant<int, 4>{});
+    }
+}
+// Tokens of an item: as many as leave about eight CTAs per SM, so that little is read twice.
+int conv_span(const SsdConvArgs& a, int channel_blocks, int least, int most) {
+    const long long total = a.cu_seqlens ? a.tokens : a.tokens * a.rows;
+    int span = most;
+    while (span > least && total / span * channel_blocks < 8LL * sm_count()) span /= 2;
+    return span;
+}
+template <class T>
+constexpr int kConvVec = 16 / static_cast<int>(sizeof(T));  // forward and step: 16 bytes
+constexpr int kConvGradVec = 4;                              // four rows of W registers per channel: 8 or 16 bytes
+ConvDims conv_grad_dims(const SsdConvArgs& a) {
+    const int blocks = (a.channels + kConvThreads * kConvGradVec - 1) / (kConvThreads * kConvGradVec);
+    return ConvDims{{a.cu_seqlens, a.tokens, a.rows, conv_span(a, blocks, 16, 128)}, blocks};
+}
+// CTAs per channel block: what the SMs hold at a time (four of them each, by registers).
+int conv_slices(const ConvDims& d) {
+    const long long items = d.map.items(), fill = (4LL * sm_count() + d.channel_blocks - 1) / d.channel_blocks;
+    return static_cast<int>(items < fill ? items : fill);
+}
+
+}  // namespace
+
+}  // namespace ssd
+
+extern "C" int ssd_short_conv_fwd(const SsdConvArgs* args, ssd_stream_t stream) {
+    using namespace ssd;
+    if (args == nullptr) return SSD_ERR_NULL;
+    const SsdConvArgs& a = *args;
+    if (const int rc = conv_check(a); rc != SSD_OK) return rc;
+    if (!a.out && a.tokens > 0) return SSD_ERR_NULL;
+    return with_type(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        constexpr int V = kConvVec<T>;
+        const int channel_blocks = (a.channels + kConvThreads * V - 1) / (kConvThreads * V);
+        const ConvDims d{{a.cu_seqlens, a.tokens, a.rows, conv_span(a, channel_blocks, 8, 32)}, channel_blocks};
+        const long long blocks = d.map.items() * channel_blocks;
+        if (blocks > 0x7fffffffLL) return static_cast<int>(SSD_ERR_RANGE);
+        const bool vector = aligned16(a.x, a.initial_state, a.out, a.final_state) && multiple_of(a.channels, V) &&
+                            multiple_of(a.batch_stride, V) && multiple_of(a.token_stride, V);
+        return with_width(a.width, [&](auto w) {
+            constexpr int W = decltype(w)::value;
+            launch_plain(vector ? conv_fwd_kernel<T, V, W, true> : conv_fwd_kernel<T, V, W, false>, static_cast<unsigned>(blocks),
+                         kConvThreads, 0, reinterpret_cast<cudaStream_t>(stream), a, d);
+            return launch_status();
+        });
+    });
+}
+
+extern "C" size_t ssd_short_conv_work_bytes(const SsdConvArgs* args) {
+    using namespace ssd;
+    if (args == nullptr || conv_check(*args) != SSD_OK) return 0;
+    return sizeof(float) * conv_slices(conv_grad_dims(*args)) * static_cast<size_t>(args->width + 1) * args->channels;
+}
+
+extern "C" int ssd_short_conv_bwd(const SsdConvGradArgs* args, ssd_stream_t stream) {
+    using namespace ssd;
+    if (args == nullptr) return SSD_ERR_NULL;
+    const SsdConvGradArgs& g = *args;
+    const SsdConvArgs& a = g.forward;
+    if (const int rc = conv_check(a); rc != SSD_OK) return rc;
+    if ((a.tokens > 0 && (!g.dout || !g.dx)) || (g.dweight && !g.work) || (g.dbias && !g.dweight)) return SSD_ERR_NULL;
+    const ConvDims d = conv_grad_dims(a);
+    const int slices = conv_slices(d);
+    const long long blocks = static_cast<long long>(slices) * d.channel_blocks;
+    if (blocks > 0x7fffffffLL) return SSD_ERR_RANGE;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return with_type(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        constexpr int V = kConvGradVec;
+        const bool vector = aligned_to(sizeof(T) * V, a.x, a.initial_state, g.dout, g.dfinal, g.dx, g.dinitial) &&
+                            multiple_of(a.channels, V) && multiple_of(a.batch_stride, V) && multiple_of(a.token_stride, V);
+        const int rc = with_width(a.width, [&](auto w) {
+            constexpr int W = decltype(w)::value;
+            launch_plain(vector ? conv_bwd_kernel<T, V, W, true> : conv_bwd_kernel<T, V, W, false>, static_cast<unsigned>(blocks),
+                         kConvThreads, 0, st, g, d, slices);
+            return launch_status();
+        });
+        if (rc != SSD_OK || g.dweight == nullptr) return rc;
+        const long long cols = static_cast<long long>(a.channels) * (a.width + 1);
+        launch_plain(conv_dw_kernel<T>, static_cast<unsigned>((cols + kSumCols - 1) / kSumCols), kSumCols * kSumRows, 0, st, g.work,
+                     static_cast<long long>(slices), a.channels, a.width, g.dweight, g.dbias, a.weight_f32);
+        return launch_status();
+    });
+}
+
+extern "C" int ssd_short_conv_step(const SsdConvStepArgs* args, ssd_stream_t stream) {
+    using namespace ssd;
+    if (args == nullptr) return SSD_ERR_NULL;
+    const SsdConvStepArgs& a = *args;
+    if (a.rows <= 0 || a.channels <= 0 || a.slot_count <= 0 || a.x_stride < 0 || a.state_stride < 0 || a.state_out_stride < 0 ||
+        (a.slots == nullptr && a.slot_count < a.rows))
+        return SSD_ERR_SHAPE;
+    if (a.width < 2 || a.width > 4) return SSD_ERR_UNSUPPORTED;
+    if (!a.x || !a.weight || !a.state || !a.state_out || !a.out) return SSD_ERR_NULL;
+    return with_type(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        constexpr int V = kConvVec<T>;
+        const int channel_blocks = (a.channels + kConvThreads * V - 1) / (kConvThreads * V);
+        const long long blocks = static_cast<long long>(a.rows) * channel_blocks;
+        if (blocks > 0x7fffffffLL) return static_cast<int>(SSD_ERR_RANGE);
+        const bool vector = aligned16(a.x, a.state, a.state_out, a.out) && multiple_of(a.channels, V) &&
+                            multiple_of(a.x_stride, V) && multiple_of(a.state_stride, V) && multiple_of(a.state_out_stride, V);
+        return with_width(a.width, [&](auto w) {
+            constexpr int W = decltype(w)::value;
+            launch_plain(vector ? conv_step_kernel<T, V, W, true> : conv_step_kernel<T, V, W, false>,
+                         static_cast<unsigned>(blocks), kConvThreads, 0, reinterpret_cast<cudaStream_t>(stream), a, channel_blocks);
+            return launch_status();
+        });
+    });
+}

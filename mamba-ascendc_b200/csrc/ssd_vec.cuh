@@ -1,0 +1,204 @@
+// Element types of the operators that take more than fp32 (short convolution, selective scan, norm) and their loads and
+// stores: a thread owns V consecutive elements and holds them in fp32.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ssd_host.h"
+
+namespace ssd {
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <class T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// The plain vector of BYTES bytes.
+template <int BYTES>
+struct Bits;
+template <>
+struct Bits<2> { using type = unsigned short; };
+template <>
+struct Bits<4> { using type = unsigned int; };
+template <>
+struct Bits<8> { using type = uint2; };
+template <>
+struct Bits<16> { using type = uint4; };
+
+// V elements as they lie in memory; V * sizeof(T) is 4, 8, 16 or a multiple of 16.
+template <class T, int V>
+struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) * V) Pack {
+    T v[V];
+};
+
+// V elements from p, n of them in range (the rest zero).  VECTOR: p is aligned for the whole vector and n is 0 or V.
+template <bool VECTOR, int V, class T>
+__device__ __forceinline__ void load_f(float (&f)[V], const T* p, int n) {
+    if constexpr (VECTOR) {
+        Pack<T, V> raw;
+        if (n > 0) {
+            constexpr int kStep = sizeof(raw) < 16 ? sizeof(raw) : 16;
+            using B = typename Bits<kStep>::type;
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(sizeof(raw)) / kStep; ++i)
+                reinterpret_cast<B*>(&raw)[i] = reinterpret_cast<const B*>(p)[i];
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = n > 0 ? to_f(raw.v[i]) : 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = i < n ? to_f(p[i]) : 0.f;
+    }
+}
+template <bool VECTOR, int V, class T>
+__device__ __forceinline__ void store_f(T* p, const float (&f)[V], int n) {
+    if constexpr (VECTOR) {
+        if (n <= 0) return;
+        Pack<T, V> raw;
+#pragma unroll
+        for (int i = 0; i < V; ++i) raw.v[i] = from_f<T>(f[i]);
+        constexpr int kStep = sizeof(raw) < 16 ? sizeof(raw) : 16;
+        using B = typename Bits<kStep>::type;
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(raw)) / kStep; ++i)
+            reinterpret_cast<B*>(p)[i] = reinterpret_cast<const B*>(&raw)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) p[i] = from_f<T>(f[i]);
+    }
+}
+
+// Parameters come in fp32 or in the activations' type, by a flag that is the same for every thread.
+template <class T>
+__device__ __forceinline__ float load_param(const void* p, int f32, long long i) {
+    return f32 ? static_cast<const float*>(p)[i] : to_f(static_cast<const T*>(p)[i]);
+}
+template <class T>
+__device__ __forceinline__ void store_param(void* p, int f32, long long i, float v) {
+    if (f32)
+        static_cast<float*>(p)[i] = v;
+    else
+        static_cast<T*>(p)[i] = from_f<T>(v);
+}
+
+__device__ __forceinline__ float ex2f(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+// 1 / (1 + e^-v): exact limits at both ends (e^-v overflows to infinity, whose reciprocal is 0)
+__device__ __forceinline__ float sigmoid_fast(float v) { return __fdividef(1.f, 1.f + ex2f(-v * kLog2e)); }
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// ---- sequences: a batch [rows, tokens], or packed one behind another as `cu` [rows + 1] says, cut into items of `span`
+// tokens so that an item lies in one sequence.  Sequence s has ceil(length / span) items, one if it is empty; packed, item
+// numbers start at start_s / span + s, which leaves room for them whatever the lengths, and numbers in between are idle.
+// Tokens behind the last packed sequence are one more sequence, `pad`, whose outputs are zeros.
+struct SeqMap {
+    const int* cu;
+    long long tokens;  // of a batch row, or all packed ones
+    int rows, span;
+    __host__ __device__ long long per_row() const { return tokens > span ? (tokens + span - 1) / span : 1; }
+    __host__ __device__ long long items() const { return cu == nullptr ? per_row() * rows : tokens / span + rows + 1; }
+    // start of sequence s; whatever `cu` holds, nothing lies outside the tokens
+    __device__ long long start(int s) const {
+        if (s == 0) return 0;
+        const long long v = cu[s];
+        return v < 0 ? 0 : v > tokens ? tokens : v;
+    }
+};
+struct Span {
+    int seq, seg;
+    bool pad, first, last;
+    long long origin;  // packed: first token of the sequence; batch: 0
+    int len, t0, t1;   // tokens of the sequence, and of this item
+};
+// Called by all threads of the CTA; false for an idle item.
+__device__ __forceinline__ bool locate(const SeqMap& m, long long item, Span& s) {
+    if (m.cu == nullptr) {
+        const long long per = m.per_row();
+        s.seq = static_cast<int>(item / per);
+        s.seg = static_cast<int>(item - s.seq * per);
+        s.origin = 0;
+        s.len = static_cast<int>(m.tokens);
+        s.pad = false;
+    } else {
+        int below = 0;  // sequences (the padding included) whose items start at or before this one
+        for (int base = 0; base <= m.rows; base += blockDim.x) {
+            const int q = base + threadIdx.x;
+            below += __syncthreads_count(q <= m.rows && m.start(q) / m.span + q <= item);
+        }
+        s.seq = max(below - 1, 0);
+        s.pad = s.seq == m.rows;
+        s.origin = m.start(s.seq);
+        const long long end = s.pad ? m.tokens : m.start(s.seq + 1);
+        s.len = static_cast<int>(max(end - s.origin, 0LL));
+        const long long seg = item - (s.origin / m.span + s.seq);
+        if (seg < 0 || (seg > 0 && seg * m.span >= s.len)) return false;
+        s.seg = static_cast<int>(seg);
+    }
+    s.t0 = s.seg * m.span;
+    s.t1 = min(s.len - s.t0, m.span) + s.t0;
+    s.first = s.seg == 0;
+    s.last = s.t1 == s.len;
+    return true;
+}
+// Row of token t: the distance in elements from the tensor's start.
+__device__ __forceinline__ long long token_row(const SeqMap& m, const Span& s, long long batch_stride, long long token_stride,
+                                               int t) {
+    return (m.cu == nullptr ? s.seq * batch_stride : 0) + (s.origin + t) * token_stride;
+}
+
+// ---- sums over the rows of a table [rows][cols] in a fixed order: the second half of gradients of parameters.
+// Cell (r, c) of `out` gets the sum of column `col`; StoreCol(col, sum) writes it.
+constexpr int kSumCols = 32, kSumRows = 32;
+template <class StoreCol>
+__device__ __forceinline__ void column_sums(const float* table, long long rows, long long cols, StoreCol store) {
+    __shared__ float part[kSumRows][kSumCols];
+    const long long c = static_cast<long long>(blockIdx.x) * kSumCols + threadIdx.x % kSumCols;
+    const int r0 = threadIdx.x / kSumCols;
+    float sum = 0.f;
+    if (c < cols) {
+#pragma unroll 8
+        for (long long r = r0; r < rows; r += kSumRows) sum += table[r * cols + c];
+    }
+    part[r0][threadIdx.x % kSumCols] = sum;
+    __syncthreads();
+    if (r0 == 0 && c < cols) {
+        for (int r = 1; r < kSumRows; ++r) sum += part[r][threadIdx.x];
+        store(c, sum);
+    }
+}
+
+// `f` with the element type that `dtype` names.
+template <class F>
+int with_type(int dtype, F f) {
+    switch (dtype) {
+        case SSD_F32: return f(float{});
+        case SSD_BF16: return f(__nv_bfloat16{});
+        case SSD_F16: return f(__half{});
+        default: return SSD_ERR_UNSUPPORTED;
+    }
+}
+inline bool multiple_of(long long v, long long m) { return v % m == 0; }
+template <class... P>
+inline bool aligned_to(size_t bytes, const P*... p) {
+    return ((reinterpret_cast<uintptr_t>(p) | ... | uintptr_t{0}) & (bytes - 1)) == 0;
+}
+
+}  // namespace ssd
