@@ -371,6 +371,53 @@ typedef struct SsdConvStepArgs {
 } SsdConvStepArgs;
 int ssd_short_conv_step(const SsdConvStepArgs* args, ssd_stream_t stream);
 
+/* Selective scan: a decay for every channel and state column,
+ *   h_t[c,n] = exp(dt_t[c] A[c,n]) h_{t-1}[c,n] + dt_t[c] x_t[c] B_t[g,n] ;  out_t[c] = (sum_n C_t[g,n] h_t[c,n] + D[c] x_t[c]) silu(z_t[c])
+ * with dt = softplus(raw + dt_bias) (or raw + dt_bias) and g = c / (channels / groups).  x, dt, z [rows, tokens, channels] and B, C [rows,
+ * tokens, groups, dstate] in the activations' type, the rest fp32: A [channels, dstate], D and dt_bias [channels] (null = none), states
+ * [rows, channels, dstate].  dstate up to 128.
+ * Strides: batch, token and, for B and C, group.  checkpoints (null = not wanted): the states that backward starts from,
+ * ssd_selective_scan_checkpoint_bytes().  work: ssd_selective_scan_work_bytes(), null where that is 0. */
+typedef struct SsdScanArgs {
+    const void *x, *dt, *z, *bm, *cm;
+    const float *A, *D, *dt_bias, *initial_state;
+    const int32_t* cu_seqlens;
+    void* out;
+    float *final_state, *checkpoints, *work;
+    int64_t tokens, x_strides[2], dt_strides[2], z_strides[2], b_strides[3], c_strides[3];
+    int32_t rows, channels, dstate, groups, dtype, softplus;
+} SsdScanArgs;
+size_t ssd_selective_scan_work_bytes(const SsdScanArgs* args);
+size_t ssd_selective_scan_checkpoint_bytes(const SsdScanArgs* args);
+int ssd_selective_scan_fwd(const SsdScanArgs* args, ssd_stream_t stream);
+
+/* Its gradients from dout (contiguous; out itself is not read) and dfinal (null = zeros), with the forward call's checkpoints.
+ * dx, ddt, dz, dbm, dcm contiguous in the activations' type, the rest fp32; dz goes with z, dD with D, d_dt_bias with dt_bias, dinitial
+ * null = not wanted.  work: ssd_selective_scan_grad_work_bytes(). */
+typedef struct SsdScanGradArgs {
+    SsdScanArgs forward;
+    const void* dout;
+    const float* dfinal;
+    void *dx, *ddt, *dz, *dbm, *dcm;
+    float *dA, *dD, *d_dt_bias, *dinitial, *work;
+} SsdScanGradArgs;
+size_t ssd_selective_scan_grad_work_bytes(const SsdScanArgs* args);
+int ssd_selective_scan_bwd(const SsdScanGradArgs* args, ssd_stream_t stream);
+
+/* One token of each of `rows` sequences: x, dt, z [rows, channels] and B, C [rows, groups, dstate], rows the given strides apart
+ * (b_strides, c_strides: row and group), states [slots, channels, dstate] fp32 with slots state_stride (state_out_stride)
+ * apart.  Slots as in ssd_short_conv_step. */
+typedef struct SsdScanStepArgs {
+    const void *x, *dt, *z, *bm, *cm;
+    const float *A, *D, *dt_bias, *state;
+    const int32_t* slots;
+    float* state_out;
+    void* out;
+    int64_t x_stride, dt_stride, z_stride, b_strides[2], c_strides[2], state_stride, state_out_stride;
+    int32_t rows, slot_count, channels, dstate, groups, dtype, softplus;
+} SsdScanStepArgs;
+int ssd_selective_scan_step(const SsdScanStepArgs* args, ssd_stream_t stream);
+
 /* ---------------------------------------------------------------- forward without any allocation
  *
  * No counterpart in the reference (its host functions allocate outputs and workspace through the

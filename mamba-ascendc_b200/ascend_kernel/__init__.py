@@ -8,6 +8,8 @@ from .mamba2 import (SavedTensorStats, check_status, mamba2_ssd_fwd, mamba_chunk
                      set_save_policy, set_state_scan)
 from .norm import rms_norm, rms_norm_quant
 from .conv import short_conv, short_conv_step
+from .selective import selective_scan, selective_scan_step
 
 __all__ = ["mamba2_ssd_fwd", "mamba_chunk_scan_combined", "check_status", "set_save_policy", "set_state_scan",
-           "SavedTensorStats", "rms_norm", "rms_norm_quant", "short_conv", "short_conv_step"]
+           "SavedTensorStats", "rms_norm", "rms_norm_quant", "short_conv", "short_conv_step",
+           "selective_scan", "selective_scan_step"]

@@ -72,6 +72,15 @@ SsdConvGradArgs = _record("SsdConvGradArgs", (SsdConvArgs, "forward"), (_P, "dou
 SsdConvStepArgs = _record("SsdConvStepArgs", (_P, "x weight bias state slots state_out out"),
                           (_I64, "x_stride state_stride state_out_stride"),
                           (_I32, "rows slot_count channels width dtype weight_f32 silu"))
+SsdScanArgs = _record("SsdScanArgs", (_P, "x dt z bm cm A D dt_bias initial_state cu_seqlens out final_state checkpoints work"),
+                      (_I64, "tokens"), (_I64 * 2, "x_strides dt_strides z_strides"), (_I64 * 3, "b_strides c_strides"),
+                      (_I32, "rows channels dstate groups dtype softplus"))
+SsdScanGradArgs = _record("SsdScanGradArgs", (SsdScanArgs, "forward"),
+                          (_P, "dout dfinal dx ddt dz dbm dcm dA dD d_dt_bias dinitial work"))
+SsdScanStepArgs = _record("SsdScanStepArgs", (_P, "x dt z bm cm A D dt_bias state slots state_out out"),
+                          (_I64, "x_stride dt_stride z_stride"), (_I64 * 2, "b_strides c_strides"),
+                          (_I64, "state_stride state_out_stride"),
+                          (_I32, "rows slot_count channels dstate groups dtype softplus"))
 
 
 def library_path() -> Path:
@@ -142,6 +151,12 @@ SIGNATURES = {
     "ssd_short_conv_work_bytes": (ctypes.c_size_t, [ctypes.POINTER(SsdConvArgs)]),
     "ssd_short_conv_bwd": (ctypes.c_int, [ctypes.POINTER(SsdConvGradArgs), _p]),
     "ssd_short_conv_step": (ctypes.c_int, [ctypes.POINTER(SsdConvStepArgs), _p]),
+    "ssd_selective_scan_work_bytes": (ctypes.c_size_t, [ctypes.POINTER(SsdScanArgs)]),
+    "ssd_selective_scan_checkpoint_bytes": (ctypes.c_size_t, [ctypes.POINTER(SsdScanArgs)]),
+    "ssd_selective_scan_fwd": (ctypes.c_int, [ctypes.POINTER(SsdScanArgs), _p]),
+    "ssd_selective_scan_grad_work_bytes": (ctypes.c_size_t, [ctypes.POINTER(SsdScanArgs)]),
+    "ssd_selective_scan_bwd": (ctypes.c_int, [ctypes.POINTER(SsdScanGradArgs), _p]),
+    "ssd_selective_scan_step": (ctypes.c_int, [ctypes.POINTER(SsdScanStepArgs), _p]),
     "ssd_use_state_scan": (ctypes.c_int, [_shape_p, ctypes.c_int]),
     "ssd_forward_work_bytes": (ctypes.c_size_t, [_shape_p]),
     "ssd_backward_work_bytes": (ctypes.c_size_t, [_shape_p, ctypes.c_int, ctypes.c_int]),

@@ -1,0 +1,116 @@
+// Shared by the kernels of the selective scan (ssd_selective_fwd.cu, _bwd.cu, _step.cu).
+#pragma once
+
+#include "ssd_vec.cuh"
+
+namespace ssd {
+
+constexpr int kScanMaxState = 128;
+constexpr int kScanCheckpoint = 64;  // tokens between the states that backward starts from
+
+// Two fp32 values for the packed arithmetic instructions.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pack2(float lo, float hi) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(F2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ F2 exp2_2(F2 v) {
+    const float2 t = unpack2(v);
+    return pack2(ex2f(t.x), ex2f(t.y));
+}
+__device__ __forceinline__ float sum2(F2 v) {
+    const float2 t = unpack2(v);
+    return t.x + t.y;
+}
+
+// log(1 + e^v) = max(v, 0) + log1p(e) with e = e^-|v| in [0, 1]; log1p(e) = 2 atanh(e / (2 + e)) by atanh's series, whose argument
+// is at most 1/3: the first term left out is below 2^-26 of the first.  Relative accuracy also where v is very negative.
+__device__ __forceinline__ float softplus_series(float v) {
+    const float e = ex2f(-fabsf(v) * kLog2e);
+    const float s = __fdividef(e, 2.f + e), q = s * s;
+    float p = 2.f / 15.f;
+    p = fmaf(p, q, 2.f / 13.f);
+    p = fmaf(p, q, 2.f / 11.f);
+    p = fmaf(p, q, 2.f / 9.f);
+    p = fmaf(p, q, 2.f / 7.f);
+    p = fmaf(p, q, 2.f / 5.f);
+    p = fmaf(p, q, 2.f / 3.f);
+    p = fmaf(p, q, 2.f);
+    return fmaf(p, s, fmaxf(v, 0.f));
+}
+
+// The channels of a CTA lie in one group.
+struct ScanBlocks {
+    int per_cta, per_group;  // channels of a CTA, CTAs of a group
+    __host__ __device__ int count(int groups) const { return per_group * groups; }
+};
+inline ScanBlocks scan_blocks(int channels, int groups, int per_cta) {
+    const int mine = channels / groups;
+    return {per_cta, (mine + per_cta - 1) / per_cta};
+}
+struct ChannelBlock {
+    int group, first, n;  // first channel and how many there are
+};
+__device__ __forceinline__ ChannelBlock channel_block(const ScanBlocks& b, int block, int channels, int groups) {
+    const int mine = channels / groups, group = block / b.per_group, at = (block - group * b.per_group) * b.per_cta;
+    return {group, group * mine + at, min(mine - at, b.per_cta)};
+}
+
+// Two channels of a row; n of them exist.
+template <bool VECTOR, class T>
+__device__ __forceinline__ float2 load_pair(const T* p, int n) {
+    float f[2];
+    load_f<VECTOR>(f, p, n);
+    return make_float2(f[0], f[1]);
+}
+template <bool VECTOR, class T>
+__device__ __forceinline__ void store_pair(T* p, float2 v, int n) {
+    const float f[2] = {v.x, v.y};
+    store_f<VECTOR>(p, f, n);
+}
+
+inline bool scan_pairs(const SsdScanArgs& a, size_t element) {
+    const int64_t strides = a.x_strides[0] | a.x_strides[1] | a.dt_strides[0] | a.dt_strides[1] | a.z_strides[0] | a.z_strides[1];
+    return aligned_to(2 * element, a.x, a.dt, a.z, a.out) && (strides & 1) == 0 && a.channels / a.groups % 2 == 0;
+}
+inline SeqMap scan_map(const SsdScanArgs& a, int span) { return SeqMap{a.cu_seqlens, a.tokens, a.rows, span}; }
+int scan_check(const SsdScanArgs& a);
+
+// ---- long sequences of few channels are cut into segments, whose states are found in two more passes: each segment's own
+// contribution from a zero state (in either direction), then a walk over the segments.
+// work: [items][dstate][channels] states, then [items][channels] sums of dt.
+struct ScanSegments {
+    int span;           // tokens of a segment
+    long long items;    // of the map
+    bool split;         // whether any sequence can have more than one
+};
+ScanSegments scan_segments(const SsdScanArgs& a, int per_cta, int slots);
+inline size_t scan_segment_floats(const SsdScanArgs& a, const ScanSegments& s) {
+    return s.split ? static_cast<size_t>(s.items) * a.channels * (a.dstate + 1) : 0;
+}
+// Leaves in `work` each segment's state before its first token (backward: the gradient of the state behind its last one).
+int scan_segment_states(const SsdScanArgs& a, const ScanSegments& s, float* work, const void* dout, const float* dfinal,
+                        cudaStream_t stream);
+
+}  // namespace ssd

@@ -11,12 +11,13 @@ def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
 
-def near(got, want, terms, ops, what=""):
-    """|got - want| <= half a step |want| + ops 2^-24 terms (want and terms in 64 bits)."""
+def near(got, want, terms, ops, what="", flushed=0.0):
+    """|got - want| <= half a step |want| + ops 2^-24 terms (want and terms in 64 bits) + flushed, what is lost of values that
+    are too small for a normal number."""
     assert got.shape == want.shape, (what, got.shape, want.shape)
     # the smallest numbers of a type are a fixed distance apart
     floor = torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
-    bound = half_step(got.dtype) * want.abs() * (1 + 2.0 ** -6) + ops * F32 * terms + floor
+    bound = half_step(got.dtype) * want.abs() * (1 + 2.0 ** -6) + ops * F32 * terms + floor + flushed
     off = (got.double() - want).abs()
     bad = ~(off <= bound)
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((off / bound).max()):.2f} times the bound"
@@ -62,3 +63,21 @@ def norm_plain(x, weight, residual, eps):
     stream = x if residual is None else x + residual
     rstd = 1 / torch.sqrt(stream.square().mean(-1, keepdim=True) + eps)
     return stream * rstd * weight, stream, rstd
+
+
+def scan_plain(x, dt, A, B, C, D, z, dt_bias, softplus, start):
+    """selective_scan of one batch, token by token in x's own type; (out, final)."""
+    per = x.shape[2] // B.shape[2]
+    B, C = (t.repeat_interleave(per, 2) for t in (B, C))
+    step = dt if dt_bias is None else dt + dt_bias
+    if softplus:
+        step = torch.logaddexp(step, torch.zeros_like(step))
+    h = x.new_zeros(x.shape[0], *A.shape) if start is None else start
+    y = []
+    for t in range(x.shape[1]):
+        h = torch.exp(step[:, t, :, None] * A) * h + (step[:, t] * x[:, t])[..., None] * B[:, t]
+        y.append((h * C[:, t]).sum(-1))
+    y = torch.stack(y, 1)
+    if D is not None:
+        y = y + D * x
+    return (y if z is None else y * silu(z)), h
