@@ -47,7 +47,9 @@ __device__ __forceinline__ Reduced reduce_row(float sum, float top, int tpr, flo
     return {sum, top};
 }
 
-template <class T, class R, int ITER, bool VECTOR, bool QUANT>
+enum NormOut { kPlain, kRowScale, kGroupScale, kOneScale };
+
+template <class T, class R, int ITER, bool VECTOR, NormOut kOut>
 __global__ void __launch_bounds__(kNormThreads)
 norm_fwd_kernel(const SsdNormArgs a, int tpr) {
     constexpr int VEC = kNormVec<T>;
@@ -57,14 +59,15 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
     const bool live = row < a.rows;
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     const R* res = static_cast<const R*>(a.residual) + row * a.residual_stride;
-    float v[ITER][VEC], w[ITER][VEC];
-    float r[ITER][VEC];
+    Pack<T, VEC> xr[ITER];
+    Pack<R, VEC> rr[ITER];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
         const int c = (at + i * tpr) * VEC, n = live ? min(a.width - c, VEC) : 0;
-        load_f<VECTOR>(v[i], x + c, n);
-        if (a.residual != nullptr) load_f<VECTOR>(r[i], res + c, n);
+        load_raw<VECTOR, false>(xr[i], x + c, n);
+        if (a.residual != nullptr) load_raw<VECTOR, false>(rr[i], res + c, n);
     }
+    float v[ITER][VEC], w[ITER][VEC];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
         const int c = (at + i * tpr) * VEC, n = min(a.width - c, VEC);
@@ -77,22 +80,24 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
         const int c = (at + i * tpr) * VEC, n = live ? min(a.width - c, VEC) : 0;
+        unpack(v[i], xr[i]);
         if (a.residual != nullptr) {
+            float r[VEC];
+            unpack(r, rr[i]);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i][j] += r[i][j];
+            for (int j = 0; j < VEC; ++j) v[i][j] += r[j];
             store_f<VECTOR>(static_cast<R*>(a.stream) + row * a.width + c, v[i], n);
         }
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             sum = fmaf(v[i][j], v[i][j], sum);
-            if (QUANT) top = max_nan(top, fabsf(v[i][j] * w[i][j]));
+            if (kOut == kRowScale) top = max_nan(top, fabsf(v[i][j] * w[i][j]));
         }
     }
-    const bool row_scale = QUANT && a.static_scale == nullptr && a.group == 0;
-    const Reduced red = QUANT ? reduce_row<true>(sum, top, tpr, part) : reduce_row<false>(sum, 0.f, tpr, part);
+    const Reduced red = reduce_row<kOut == kRowScale>(sum, top, tpr, part);
     const float rstd = rsqrtf(red.sum / static_cast<float>(a.width) + a.eps);
     if (a.rstd != nullptr && live && at == 0) a.rstd[row] = rstd;
-    if constexpr (!QUANT) {
+    if constexpr (kOut == kPlain) {
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int c = (at + i * tpr) * VEC, n = live ? min(a.width - c, VEC) : 0;
@@ -102,8 +107,8 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
         }
     } else {
         float scale = 1.f;
-        if (a.static_scale != nullptr) scale = *static_cast<const float*>(a.static_scale);
-        if (row_scale) {
+        if (kOut == kOneScale) scale = *static_cast<const float*>(a.static_scale);
+        if (kOut == kRowScale) {
             // rstd is positive, so the largest |v w| is the largest |out| but for rstd
             scale = red.top * rstd / 448.f;
             if (scale == 0.f) scale = 1.f;
@@ -115,7 +120,7 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
             float y[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) y[j] = v[i][j] * rstd * w[i][j];
-            if (a.group != 0 && a.static_scale == nullptr) {
+            if (kOut == kGroupScale) {
                 // a group is group / VEC neighbouring lanes, a power of two that divides 32
                 float m = 0.f;
 #pragma unroll
@@ -126,14 +131,19 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
                 if (n > 0 && c % a.group == 0) a.scales[row * (a.width / a.group) + c / a.group] = scale;
             }
             // a reciprocal, but for scales so small that it would overflow
-            const bool tiny = fabsf(scale) < 1e-30f;
-            const float inv = tiny ? 1.f : 1.f / scale;
+            if (fabsf(scale) < 1e-30f) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) y[j] = y[j] / scale;
+            } else {
+                const float inv = 1.f / scale;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) y[j] *= inv;
+            }
             alignas(8) unsigned char q[VEC];
 #pragma unroll
-            for (int j = 0; j < VEC; j += 2) {
-                const float2 t = tiny ? make_float2(y[j] / scale, y[j + 1] / scale) : make_float2(y[j] * inv, y[j + 1] * inv);
-                *reinterpret_cast<unsigned short*>(q + j) = __nv_cvt_float2_to_fp8x2(t, __NV_SATFINITE, __NV_E4M3);
-            }
+            for (int j = 0; j < VEC; j += 2)
+                *reinterpret_cast<unsigned short*>(q + j) =
+                    __nv_cvt_float2_to_fp8x2(make_float2(y[j], y[j + 1]), __NV_SATFINITE, __NV_E4M3);
             unsigned char* dst = static_cast<unsigned char*>(a.q) + row * a.width + c;
             if constexpr (VECTOR) {
                 using B = typename Bits<VEC>::type;
@@ -149,66 +159,81 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
 
 // CTAs walk the rows at a distance of the grid, so that a thread keeps its columns and sums their share of dw in registers;
 // the CTA's rows are added up in shared memory and leave as one row of `work`, which norm_dw_kernel sums in a fixed order.
+// The next row's loads are in flight under this one's sums.
 template <class T, class R, int ITER, bool VECTOR>
-__global__ void __launch_bounds__(kNormThreads)
+__global__ void __launch_bounds__(kNormThreads, ITER == 1 ? 2 : 1)
 norm_bwd_kernel(const SsdNormGradArgs a, int tpr) {
     constexpr int VEC = kNormVec<T>;
     __shared__ float part[2][64];
     extern __shared__ float norm_rows[];  // [rows of the CTA][width], only where there are several
     const int at = threadIdx.x % tpr, rows_here = blockDim.x / tpr, mine = threadIdx.x / tpr;
-    float w[ITER][VEC], dw[ITER][VEC];
+    float dw[ITER][VEC];
 #pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-        const int c = (at + i * tpr) * VEC, n = min(a.width - c, VEC);
-        if (a.weight_f32)
-            load_f<VECTOR>(w[i], static_cast<const float*>(a.weight) + c, n);
-        else
-            load_f<VECTOR>(w[i], static_cast<const T*>(a.weight) + c, n);
+    for (int i = 0; i < ITER; ++i)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) dw[i][j] = 0.f;
-    }
-    int parity = 0;
-    for (long long first = static_cast<long long>(blockIdx.x) * rows_here; first < a.rows;
-         first += static_cast<long long>(gridDim.x) * rows_here) {
-        const long long row = first + mine;
+    Pack<R, VEC> vr[ITER], sr[ITER];
+    Pack<T, VEC> gr[ITER], ur[ITER];
+    float rstd_next = 0.f;
+    const auto request = [&](long long row) {
         const bool live = row < a.rows;
-        const float rstd = live ? a.rstd[row] : 0.f;
-        float v[ITER][VEC], g[ITER][VEC], s[ITER][VEC];
+        rstd_next = live ? __ldg(a.rstd + row) : 0.f;
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int c = (at + i * tpr) * VEC, n = live ? min(a.width - c, VEC) : 0;
-            load_f<VECTOR>(v[i], static_cast<const R*>(a.stream) + row * a.stream_stride + c, n);
-            load_f<VECTOR>(g[i], static_cast<const T*>(a.dout) + row * a.dout_stride + c, n);
+            load_raw<VECTOR, false>(vr[i], static_cast<const R*>(a.stream) + row * a.stream_stride + c, n);
+            load_raw<VECTOR, false>(gr[i], static_cast<const T*>(a.dout) + row * a.dout_stride + c, n);
             if (a.dstream != nullptr)
-                load_f<VECTOR>(s[i], static_cast<const R*>(a.dstream) + row * a.dstream_stride + c, n);
-            if (a.addend != nullptr) {
-                float u[VEC];
-                load_f<VECTOR>(u, static_cast<const T*>(a.addend) + row * a.addend_stride + c, n);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[i][j] += u[j];
-            }
+                load_raw<VECTOR, false>(sr[i], static_cast<const R*>(a.dstream) + row * a.dstream_stride + c, n);
+            if (a.addend != nullptr)
+                load_raw<VECTOR, false>(ur[i], static_cast<const T*>(a.addend) + row * a.addend_stride + c, n);
         }
+    };
+    const long long step = static_cast<long long>(gridDim.x) * rows_here;
+    request(static_cast<long long>(blockIdx.x) * rows_here + mine);
+    int parity = 0;
+    for (long long first = static_cast<long long>(blockIdx.x) * rows_here; first < a.rows; first += step) {
+        const long long row = first + mine;
+        const bool live = row < a.rows;
+        const float rstd = rstd_next;
+        float v[ITER][VEC], g[ITER][VEC];
+        Pack<R, VEC> s[ITER];
         float dot = 0.f;
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
+            const int c = (at + i * tpr) * VEC, n = min(a.width - c, VEC);
+            float w[VEC];
+            if (a.weight_f32)
+                load_f<VECTOR>(w, static_cast<const float*>(a.weight) + c, n);
+            else
+                load_f<VECTOR>(w, static_cast<const T*>(a.weight) + c, n);
+            unpack(v[i], vr[i]);
+            unpack(g[i], gr[i]);
+            s[i] = sr[i];
+            if (a.addend != nullptr) {
+                float u[VEC];
+                unpack(u, ur[i]);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[i][j] += u[j];
+            }
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 v[i][j] *= rstd;
                 dw[i][j] = fmaf(g[i][j], v[i][j], dw[i][j]);
-                g[i][j] *= w[i][j];
+                g[i][j] *= w[j];
                 dot = fmaf(g[i][j], v[i][j], dot);
             }
         }
+        if (first + step < a.rows) request(row + step);
         const float mean = reduce_row<false>(dot, 0.f, tpr, part[parity]).sum / static_cast<float>(a.width);
         parity ^= 1;
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int c = (at + i * tpr) * VEC, n = live ? min(a.width - c, VEC) : 0;
+            float d[VEC] = {};
+            if (a.dstream != nullptr) unpack(d, s[i]);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                g[i][j] = rstd * fmaf(-v[i][j], mean, g[i][j]);
-                if (a.dstream != nullptr) g[i][j] += s[i][j];
-            }
+            for (int j = 0; j < VEC; ++j) g[i][j] = fmaf(rstd, fmaf(-v[i][j], mean, g[i][j]), d[j]);
             store_f<VECTOR>(static_cast<T*>(a.dx) + row * a.width + c, g[i], n);
             if (a.dresidual != nullptr) store_f<VECTOR>(static_cast<R*>(a.dresidual) + row * a.width + c, g[i], n);
         }
@@ -249,8 +274,9 @@ norm_dw_kernel(const float* table, long long rows, int width, void* dweight, int
 struct NormGeometry {
     int tpr, iter, rows_here;
 };
-// Threads per row and vectors per thread.  Rows of up to 128 vectors are a warp's; of longer ones a thread takes one vector where
-// there are few rows (latency counts) and up to `most` where they fill the GPU anyway (fewer threads to reduce over).
+// Threads per row and vectors per thread.  Rows of up to 32 vectors per thread's share are a warp's; of longer ones a thread
+// takes one vector where there are few rows (latency counts) and up to `most` where they fill the GPU anyway (fewer threads
+// to reduce over).
 NormGeometry norm_geometry(long long rows, int width, int vec, int most) {
     const int vecs = (width + vec - 1) / vec;
     const bool many = rows >= 8LL * sm_count();
@@ -266,10 +292,14 @@ NormGeometry norm_geometry(long long rows, int width, int vec, int most) {
     g.rows_here = g.tpr == 32 && many ? 8 : 1;
     return g;
 }
-constexpr int kNormGradIter = 2;
+// Backward: two vectors per thread only where a row is one warp's or would take more than a CTA's threads.
+NormGeometry norm_grad_geometry(long long rows, int width, int vec) {
+    return norm_geometry(rows, width, vec, (width + vec - 1) / vec <= 64 ? 2 : 1);
+}
 unsigned norm_bwd_grid(long long rows, const NormGeometry& g) {
     const long long all = (rows + g.rows_here - 1) / g.rows_here;
-    const long long resident = static_cast<long long>(sm_count()) * (1024 / (g.tpr * g.rows_here));
+    const int threads = g.tpr * g.rows_here;
+    const long long resident = static_cast<long long>(sm_count()) * ((g.iter == 1 ? 1024 : 512) / threads);
     return static_cast<unsigned>(all < resident ? all : resident);
 }
 
@@ -311,7 +341,7 @@ extern "C" int ssd_rms_norm_fwd(const SsdNormArgs* args, ssd_stream_t stream) {
         return with_residual_type<T>(a.residual_f32, [&](auto r) {
             using R = decltype(r);
             const int vec = kNormVec<T>;
-            const NormGeometry g = norm_geometry(a.rows, a.width, vec, 4);
+            const NormGeometry g = norm_geometry(a.rows, a.width, vec, quant ? 2 : 4);
             const long long blocks = (a.rows + g.rows_here - 1) / g.rows_here;
             if (blocks > 0x7fffffffLL) return static_cast<int>(SSD_ERR_RANGE);
             const bool vector = aligned16(a.x, a.residual, a.weight, a.out, a.stream, a.q) && multiple_of(a.width, vec) &&
@@ -321,10 +351,18 @@ extern "C" int ssd_rms_norm_fwd(const SsdNormArgs* args, ssd_stream_t stream) {
                 const auto launch = [&](auto kernel) {
                     launch_plain(kernel, static_cast<unsigned>(blocks), g.tpr * g.rows_here, 0, st, a, g.tpr);
                 };
-                if (quant)
-                    vector ? launch(norm_fwd_kernel<T, R, I, true, true>) : launch(norm_fwd_kernel<T, R, I, false, true>);
+                const auto with = [&](auto out) {
+                    constexpr NormOut kOut = decltype(out)::value;
+                    vector ? launch(norm_fwd_kernel<T, R, I, true, kOut>) : launch(norm_fwd_kernel<T, R, I, false, kOut>);
+                };
+                if (!quant)
+                    with(std::integral_constant<NormOut, kPlain>{});
+                else if (a.static_scale != nullptr)
+                    with(std::integral_constant<NormOut, kOneScale>{});
+                else if (a.group != 0)
+                    with(std::integral_constant<NormOut, kGroupScale>{});
                 else
-                    vector ? launch(norm_fwd_kernel<T, R, I, true, false>) : launch(norm_fwd_kernel<T, R, I, false, false>);
+                    with(std::integral_constant<NormOut, kRowScale>{});
                 return launch_status();
             });
         });
@@ -334,7 +372,7 @@ extern "C" int ssd_rms_norm_fwd(const SsdNormArgs* args, ssd_stream_t stream) {
 extern "C" size_t ssd_rms_norm_work_bytes(int64_t rows, int width, int dtype) {
     using namespace ssd;
     if (rows <= 0 || width <= 0 || width > kNormMaxWidth || dtype < SSD_F32 || dtype > SSD_F16) return 0;
-    const NormGeometry g = norm_geometry(rows, width, dtype == SSD_F32 ? 4 : 8, kNormGradIter);
+    const NormGeometry g = norm_grad_geometry(rows, width, dtype == SSD_F32 ? 4 : 8);
     return sizeof(float) * static_cast<size_t>(norm_bwd_grid(rows, g)) * width;
 }
 
@@ -352,7 +390,7 @@ extern "C" int ssd_rms_norm_bwd(const SsdNormGradArgs* args, ssd_stream_t stream
         return with_residual_type<T>(a.residual_f32, [&](auto r) {
             using R = decltype(r);
             const int vec = kNormVec<T>;
-            const NormGeometry g = norm_geometry(a.rows, a.width, vec, kNormGradIter);
+            const NormGeometry g = norm_grad_geometry(a.rows, a.width, vec);
             const unsigned grid = norm_bwd_grid(a.rows, g);
             const size_t smem = g.rows_here > 1 ? sizeof(float) * g.rows_here * a.width : 0;
             const bool vector = aligned16(a.dout, a.dstream, a.stream, a.addend, a.weight, a.dx, a.dresidual) &&

@@ -77,6 +77,10 @@ __device__ __forceinline__ ChannelBlock channel_block(const ScanBlocks& b, int b
     return {group, group * mine + at, min(mine - at, b.per_cta)};
 }
 
+template <class T>
+__device__ __forceinline__ float2 pair_f(const Pack<T, 2>& raw) {
+    return make_float2(to_f(raw.v[0]), to_f(raw.v[1]));
+}
 // Two channels of a row; n of them exist.
 template <bool VECTOR, class T>
 __device__ __forceinline__ float2 load_pair(const T* p, int n) {

@@ -37,6 +37,8 @@ size_t bwd_smem(int dstate) {
     return sizeof(float) * (2 * dstate * kRow + 4 * dstate * kBwdChannels + 2 * kWarps * kBwdChannels * (2 + 1 + 1));
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // Sums over the 32 lanes of 16 values each: a lane ends up with the sum of value `lane / 2` (both of a pair the same).  Each
 // step hands half of the values to the lane on the other side, 8 + 4 + 2 + 1 + 1 exchanges instead of 80.
 __device__ __forceinline__ float sum_lanes16(float (&v)[16], int lane) {
@@ -135,17 +137,24 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
         // ---- this warp's tokens
         F2 dt[kTokens], u[kTokens], dy[kTokens];
         float2 sum_dt = make_float2(0.f, 0.f);
+        Pack<T, 2> xr[kTokens], dr[kTokens], zr[kTokens], gr[kTokens];
 #pragma unroll
         for (int i = 0; i < kTokens; ++i) {
             const int t = tw + i, n = t < s.t1 ? pn : 0;
-            const float2 xv = load_pair<VECTOR>(x + t * a.x_strides[1], n);
-            float2 d = load_pair<VECTOR>(dtp + t * a.dt_strides[1], n);
-            float2 o = load_pair<VECTOR>(dout + static_cast<long long>(t) * a.channels, n);
+            load_raw<VECTOR, false>(xr[i], x + t * a.x_strides[1], n);
+            load_raw<VECTOR, false>(dr[i], dtp + t * a.dt_strides[1], n);
+            load_raw<VECTOR, false>(gr[i], dout + static_cast<long long>(t) * a.channels, n);
+            if (GATED) load_raw<VECTOR, false>(zr[i], z + t * a.z_strides[1], n);
+        }
+#pragma unroll
+        for (int i = 0; i < kTokens; ++i) {
+            const float2 xv = pair_f(xr[i]);
+            float2 d = pair_f(dr[i]), o = pair_f(gr[i]);
             d = make_float2(d.x + bias.x, d.y + bias.y);
             if (a.softplus) d = make_float2(softplus_series(d.x), softplus_series(d.y));
-            if (n == 0) d = make_float2(0.f, 0.f);
+            if (tw + i >= s.t1) d = make_float2(0.f, 0.f);
             if (GATED) {
-                const float2 zv = load_pair<VECTOR>(z + t * a.z_strides[1], n);
+                const float2 zv = pair_f(zr[i]);
                 o = make_float2(o.x * zv.x * sigmoid_fast(zv.x), o.y * zv.y * sigmoid_fast(zv.y));
             }
             sum_dt = make_float2(sum_dt.x + d.x, sum_dt.y + d.y);
@@ -166,13 +175,20 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
         for (int i = 0; i < kTokens; ++i) ddt2[i] = du[i] = y[i] = 0;
         const F2 total_dt = pack2(sum_dt.x, sum_dt.y);
         const float* hp = a.checkpoints + (checkpoint0 + t0 / kScanCheckpoint) * N * a.channels + c;
+        if (k > 0 && lane < kTokens) {  // the next chunk's rows (the tokens before) into L2
+            const int t = tw - kChunk + lane;
+            prefetch_l2(x + t * a.x_strides[1] - 2 * lane);
+            prefetch_l2(dtp + t * a.dt_strides[1] - 2 * lane);
+            prefetch_l2(dout + static_cast<long long>(t) * a.channels - 2 * lane);
+            if (GATED) prefetch_l2(z + t * a.z_strides[1] - 2 * lane);
+        }
+        Pack<float, 2> h_start;
+        load_raw<VECTOR, false>(h_start, hp, pn);  // the state that the chunk starts from, a column ahead
         for (int n = 0; n < N; ++n) {
             const int buf = n & 1;
             const F2 a2 = *reinterpret_cast<const F2*>(sa + n * kBwdChannels + 2 * lane);
-            // the state that the chunk starts from, for after the barrier
-            float2 h0 = make_float2(0.f, 0.f);
-            if (pn > 0) h0.x = hp[static_cast<long long>(n) * a.channels];
-            if (pn > 1) h0.y = hp[static_cast<long long>(n) * a.channels + 1];
+            F2 hs = pack2(h_start.v[0], h_start.v[1]);
+            if (n + 1 < N) load_raw<VECTOR, false>(h_start, hp + static_cast<long long>(n + 1) * a.channels, pn);
             float bt[kTokens], ct[kTokens];
 #pragma unroll
             for (int i = 0; i < kTokens; i += 4) {
@@ -206,19 +222,24 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
                 }
                 *at = sum;
             }
-            F2 hs = pack2(h0.x, h0.y);
-            for (int v = 0; v < w; ++v) {
-                const ulonglong2 e = *reinterpret_cast<const ulonglong2*>(ex_h + (buf * kWarps + v) * 32 + lane);
-                hs = fma2(e.x, hs, e.y);
-            }
+            // all of them loaded at once; whether a warp lies before or behind is the same for all lanes
             F2 gs = *reinterpret_cast<const F2*>(sg + (side * N + n) * kBwdChannels + 2 * lane);
-            for (int v = kWarps - 1; v > w; --v) {
-                const F2 p = *reinterpret_cast<const F2*>(ex_h + (buf * kWarps + v) * 32 + lane);
-                gs = fma2(p, gs, *reinterpret_cast<const F2*>(ex_g + (buf * kWarps + v) * 32 + lane));
+            F2 decay[kWarps], end[kWarps];
+#pragma unroll
+            for (int v = 0; v < kWarps; ++v) {
+                const F2* before = reinterpret_cast<const F2*>(ex_h + (buf * kWarps + v) * 32 + lane);
+                const F2* behind = reinterpret_cast<const F2*>(ex_g + (buf * kWarps + v) * 32 + lane);
+                decay[v] = *before;
+                end[v] = v < w ? before[1] : *behind;
             }
+#pragma unroll
+            for (int v = 0; v < kWarps - 1; ++v)
+                if (v < w) hs = fma2(decay[v], hs, end[v]);
+#pragma unroll
+            for (int v = kWarps - 1; v > 0; --v)
+                if (v > w) gs = fma2(decay[v], gs, end[v]);
             if (w == 0) {
-                const F2 p = *reinterpret_cast<const F2*>(ex_h + buf * kWarps * 32 + lane);
-                *reinterpret_cast<F2*>(sg + ((side ^ 1) * N + n) * kBwdChannels + 2 * lane) = fma2(p, gs, end_g);
+                *reinterpret_cast<F2*>(sg + ((side ^ 1) * N + n) * kBwdChannels + 2 * lane) = fma2(decay[0], gs, end_g);
             }
             float v16[16];  // dB, dC of the tokens, over this lane's channels
             {
@@ -269,12 +290,22 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
 #pragma unroll
         for (int i = 0; i < kTokens; ++i) {
             const int t = tw + i, n = t < s.t1 ? pn : 0;
-            const float2 xv = load_pair<VECTOR>(x + t * a.x_strides[1], n);
+            load_raw<VECTOR, false>(xr[i], x + t * a.x_strides[1], n);
+            load_raw<VECTOR, false>(dr[i], dtp + t * a.dt_strides[1], n);
+            if (GATED) {
+                load_raw<VECTOR, false>(zr[i], z + t * a.z_strides[1], n);
+                load_raw<VECTOR, false>(gr[i], dout + static_cast<long long>(t) * a.channels, n);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kTokens; ++i) {
+            const int t = tw + i, n = t < s.t1 ? pn : 0;
+            const float2 xv = pair_f(xr[i]);
             const float2 dv = unpack2(dt[i]), duv = unpack2(du[i]), dyv = unpack2(dy[i]), qa = unpack2(ddt2[i]);
             constexpr float kLn2 = 0.6931471805599453f;
             float2 dd = make_float2(fmaf(qa.x, kLn2, xv.x * duv.x), fmaf(qa.y, kLn2, xv.y * duv.y));
             if (a.softplus) {
-                float2 raw = load_pair<VECTOR>(dtp + t * a.dt_strides[1], n);
+                const float2 raw = pair_f(dr[i]);
                 dd.x *= sigmoid_fast(raw.x + bias.x);
                 dd.y *= sigmoid_fast(raw.y + bias.y);
             }
@@ -283,8 +314,7 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
                                make_float2(fmaf(dv.x, duv.x, skip.x * dyv.x), fmaf(dv.y, duv.y, skip.y * dyv.y)), n);
             store_pair<VECTOR>(static_cast<T*>(g.ddt) + at, dd, n);
             if (GATED) {
-                const float2 zv = load_pair<VECTOR>(z + t * a.z_strides[1], n), yv = unpack2(y[i]);
-                const float2 o = load_pair<VECTOR>(dout + static_cast<long long>(t) * a.channels, n);
+                const float2 zv = pair_f(zr[i]), yv = unpack2(y[i]), o = pair_f(gr[i]);
                 const float gx = sigmoid_fast(zv.x), gy = sigmoid_fast(zv.y);
                 store_pair<VECTOR>(static_cast<T*>(g.dz) + at,
                                    make_float2(o.x * fmaf(skip.x, xv.x, yv.x) * gx * fmaf(zv.x, 1.f - gx, 1.f),

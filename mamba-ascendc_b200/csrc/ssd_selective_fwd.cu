@@ -112,30 +112,29 @@ selective_walk_kernel(const SsdScanArgs a, const ScanLaunch l) {
         if (a.D != nullptr) skip = make_float2(a.D[cb.first + 2 * pair], pn > 1 ? a.D[cb.first + 2 * pair + 1] : 0.f);
     }
     const int shared_each = kShared / l.cg;  // of them
-    float2 xr[kPairs], dr[kPairs], zr[kPairs];
-    float br[kShared];
+    Pack<T, 2> xr[kPairs], dr[kPairs], zr[kPairs];
+    Pack<T, 1> br[kShared];
     auto request = [&](int t0) {
 #pragma unroll
         for (int p = 0; p < kPairs; ++p) {
             const int t = t0 + first_row + p * row_step;
             const int n = t < s.t1 ? pn : 0;
-            if (!kReverse) xr[p] = load_pair<VECTOR>(x + t * a.x_strides[1] + 2 * pair, n);
-            dr[p] = load_pair<VECTOR>(dt + t * a.dt_strides[1] + 2 * pair, n);
+            load_raw<VECTOR, false>(dr[p], dt + t * a.dt_strides[1] + 2 * pair, n);
             if (kReverse) {
-                xr[p] = load_pair<VECTOR>(dout + static_cast<long long>(t) * a.channels + 2 * pair, n);
-                if (a.z != nullptr) zr[p] = load_pair<VECTOR>(z + t * a.z_strides[1] + 2 * pair, n);
+                load_raw<VECTOR, false>(xr[p], dout + static_cast<long long>(t) * a.channels + 2 * pair, n);
+                if (a.z != nullptr) load_raw<VECTOR, false>(zr[p], z + t * a.z_strides[1] + 2 * pair, n);
+            } else {
+                load_raw<VECTOR, false>(xr[p], x + t * a.x_strides[1] + 2 * pair, n);
             }
         }
 #pragma unroll
         for (int p = 0; p < kShared; ++p) {
             const int i = tid + (p / 2) * threads, t = t0 + i / kCols, n = i % kCols;
-            br[p] = 0.f;
-            if (p < shared_each && n < a.dstate && t < s.t1) {
-                if (p % 2 == 0)
-                    br[p] = to_f(bm[t * b_step + n]);
-                else if (kMode == kForward)
-                    br[p] = to_f(cm[t * a.c_strides[1] + n]);
-            }
+            const int in = p < shared_each && n < a.dstate && t < s.t1 ? 1 : 0;
+            if (p % 2 == 0)
+                load_raw<true, false>(br[p], bm + t * b_step + n, in);
+            else if (kMode == kForward)
+                load_raw<true, false>(br[p], cm + t * a.c_strides[1] + n, in);
         }
     };
     const int tiles = (s.t1 - s.t0 + kScanTile - 1) / kScanTile;
@@ -149,30 +148,35 @@ selective_walk_kernel(const SsdScanArgs a, const ScanLaunch l) {
         for (int p = 0; p < kPairs; ++p) {
             const int row = first_row + p * row_step;
             const bool in = row < nt;
-            float2 d = make_float2(dr[p].x + bias.x, dr[p].y + bias.y);
+            const float2 xv = pair_f(xr[p]);
+            float2 d = pair_f(dr[p]);
+            d = make_float2(d.x + bias.x, d.y + bias.y);
             if (a.softplus) d = make_float2(softplus_series(d.x), softplus_series(d.y));
             if (!in) d = make_float2(0.f, 0.f);  // behind the last token the state stays
             float2 u;
             if (kReverse) {
-                u = xr[p];
-                if (a.z != nullptr)
-                    u = make_float2(u.x * zr[p].x * sigmoid_fast(zr[p].x), u.y * zr[p].y * sigmoid_fast(zr[p].y));
+                u = xv;
+                if (a.z != nullptr) {
+                    const float2 zv = pair_f(zr[p]);
+                    u = make_float2(u.x * zv.x * sigmoid_fast(zv.x), u.y * zv.y * sigmoid_fast(zv.y));
+                }
             } else {
-                u = make_float2(d.x * xr[p].x, d.y * xr[p].y);
+                u = make_float2(d.x * xv.x, d.y * xv.y);
             }
-            held[p] = xr[p];
+            held[p] = xv;
             *reinterpret_cast<float4*>(&sdu[row * channels_here + 2 * pair]) = make_float4(d.x, u.x, d.y, u.y);
         }
 #pragma unroll
         for (int p = 0; p < kShared; ++p)
-            if (p < shared_each) (p % 2 == 0 ? sb : sc)[tid + (p / 2) * threads] = br[p];
+            if (p < shared_each && (p % 2 == 0 || kMode == kForward))
+                (p % 2 == 0 ? sb : sc)[tid + (p / 2) * threads] = to_f(br[p].v[0]);
         __syncthreads();
         if (k + 1 < tiles) request(tile_start(k + 1));
         if (kMode == kForward && a.z != nullptr) {
 #pragma unroll
             for (int p = 0; p < kPairs; ++p) {
                 const int t = t0 + first_row + p * row_step;
-                zr[p] = load_pair<VECTOR>(z + t * a.z_strides[1] + 2 * pair, t < s.t1 ? pn : 0);
+                load_raw<VECTOR, false>(zr[p], z + t * a.z_strides[1] + 2 * pair, t < s.t1 ? pn : 0);
             }
         }
         if (kMode == kForward && a.checkpoints != nullptr && (t0 - s.t0) % kScanCheckpoint == 0 && live) {
@@ -185,32 +189,68 @@ selective_walk_kernel(const SsdScanArgs a, const ScanLaunch l) {
                 if (n0 + j < a.dstate) dst[static_cast<long long>(n0 + j) * a.channels] = j % 2 ? v.y : v.x;
             }
         }
-        const int steps = (nt + 3) / 4 * 4;  // rows behind the last token have dt = 0
-#pragma unroll 4
-        for (int i = 0; i < steps; ++i) {
-            const int row = kReverse ? steps - 1 - i : i;
-            const float2 du = sdu[row * channels_here + mine];
-            const F2 dd = pack2(du.x, du.x), uu = pack2(du.y, du.y);
-            if (kMode != kForward) sum_dt += du.x;
-            F2 y = 0;
+        // kGroup tokens at a time, the next ones' operands on their way: nothing but the states depends on the token before.
+        // Rows behind the last token have dt = 0; groups of nothing else are left out.
+        constexpr int kGroup = NPL <= 4 ? 4 : NPL <= 8 ? 2 : 1, kGroups = kScanTile / kGroup;
+        struct Operands {
+            float2 du[kGroup];
+            ulonglong2 b[kGroup][NPL / 4], c[kGroup][NPL / 4];
+        };
+        const auto row_of = [](int i) { return kReverse ? kScanTile - 1 - i : i; };
+        const auto fetch = [&](Operands& o, int group) {
 #pragma unroll
-            for (int j = 0; j < NPL / 2; j += 2) {
-                const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sb + row * kCols + n0 + 2 * j);
-                const F2 e0 = exp2_2(mul2(dd, a2[j])), e1 = exp2_2(mul2(dd, a2[j + 1]));
-                if (kReverse) {
-                    h[j] = mul2(e0, fma2(uu, b.x, h[j]));
-                    h[j + 1] = mul2(e1, fma2(uu, b.y, h[j + 1]));
-                } else {
-                    h[j] = fma2(e0, h[j], mul2(uu, b.x));
-                    h[j + 1] = fma2(e1, h[j + 1], mul2(uu, b.y));
-                }
-                if (kMode == kForward) {
-                    const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(sc + row * kCols + n0 + 2 * j);
-                    y = fma2(cv.x, h[j], y);
-                    y = fma2(cv.y, h[j + 1], y);
+            for (int i = 0; i < kGroup; ++i) {
+                const int row = row_of(group * kGroup + i);
+                o.du[i] = sdu[row * channels_here + mine];
+#pragma unroll
+                for (int j = 0; j < NPL / 4; ++j) {
+                    o.b[i][j] = *reinterpret_cast<const ulonglong2*>(sb + row * kCols + n0 + 4 * j);
+                    if (kMode == kForward) o.c[i][j] = *reinterpret_cast<const ulonglong2*>(sc + row * kCols + n0 + 4 * j);
                 }
             }
-            if (kMode == kForward) sy[(wn * kScanTile + row) * channels_here + mine] = sum2(y);
+        };
+        Operands now, next;
+        fetch(now, 0);
+#pragma unroll
+        for (int group = 0; group < kGroups; ++group) {
+            if (!kReverse && group * kGroup >= nt) break;
+            if (group + 1 < kGroups) fetch(next, group + 1);
+            if (!kReverse || row_of(group * kGroup + kGroup - 1) < nt) {
+                F2 e[kGroup][NPL / 2];
+                float y[kGroup];
+#pragma unroll
+                for (int i = 0; i < kGroup; ++i)
+#pragma unroll
+                    for (int j = 0; j < NPL / 2; ++j) e[i][j] = exp2_2(mul2(pack2(now.du[i].x, now.du[i].x), a2[j]));
+#pragma unroll
+                for (int i = 0; i < kGroup; ++i) {
+                    const F2 uu = pack2(now.du[i].y, now.du[i].y);
+                    if (kMode != kForward) sum_dt += now.du[i].x;
+                    F2 sum = 0;
+#pragma unroll
+                    for (int j = 0; j < NPL / 4; ++j) {
+                        const ulonglong2 bv = now.b[i][j];
+                        if (kReverse) {
+                            h[2 * j] = mul2(e[i][2 * j], fma2(uu, bv.x, h[2 * j]));
+                            h[2 * j + 1] = mul2(e[i][2 * j + 1], fma2(uu, bv.y, h[2 * j + 1]));
+                        } else {
+                            h[2 * j] = fma2(e[i][2 * j], h[2 * j], mul2(uu, bv.x));
+                            h[2 * j + 1] = fma2(e[i][2 * j + 1], h[2 * j + 1], mul2(uu, bv.y));
+                        }
+                        if (kMode == kForward) {
+                            sum = fma2(now.c[i][j].x, h[2 * j], sum);
+                            sum = fma2(now.c[i][j].y, h[2 * j + 1], sum);
+                        }
+                    }
+                    y[i] = sum2(sum);
+                }
+                if (kMode == kForward) {
+#pragma unroll
+                    for (int i = 0; i < kGroup; ++i)
+                        sy[(wn * kScanTile + row_of(group * kGroup + i)) * channels_here + mine] = y[i];
+                }
+            }
+            now = next;
         }
         __syncthreads();
         if (kMode == kForward) {
@@ -226,8 +266,9 @@ selective_walk_kernel(const SsdScanArgs a, const ScanLaunch l) {
                     y.y += v.y;
                 }
                 if (a.z != nullptr) {
-                    y.x *= zr[p].x * sigmoid_fast(zr[p].x);
-                    y.y *= zr[p].y * sigmoid_fast(zr[p].y);
+                    const float2 zv = pair_f(zr[p]);
+                    y.x *= zv.x * sigmoid_fast(zv.x);
+                    y.y *= zv.y * sigmoid_fast(zv.y);
                 }
                 store_pair<VECTOR>(out + static_cast<long long>(t0 + row) * a.channels + 2 * pair, y, pn);
             }

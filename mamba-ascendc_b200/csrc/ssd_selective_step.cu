@@ -11,7 +11,8 @@ namespace {
 
 constexpr int kStepThreads = 128;
 
-// LPC lanes hold a channel's columns, four each.  VECTOR: dstate is a multiple of four and the states are aligned.
+// LPC lanes hold a channel's columns, four each.  VECTOR: dstate is a multiple of four, and states, B and C
+// are aligned for four at once.
 template <class T, int LPC, int ROWS, bool VECTOR>
 __global__ void __launch_bounds__(kStepThreads)
 selective_step_kernel(const SsdScanStepArgs a, int channel_blocks) {
@@ -23,15 +24,30 @@ selective_step_kernel(const SsdScanStepArgs a, int channel_blocks) {
     const bool live = c < a.channels;
     const int g = live ? c / (a.channels / a.groups) : 0;
 
+    // every load of the rows in flight before the first is used
     long long slot[ROWS];
-    float h[ROWS][4];
+    Pack<float, 4> hr[ROWS];
+    Pack<T, 4> br[ROWS], cr[ROWS];
+    Pack<T, 1> xr[ROWS], dr[ROWS], zr[ROWS];
+    auto request = [&](Pack<T, 1>& xv, Pack<T, 1>& dv, Pack<T, 1>& zv, Pack<T, 4>& bv, Pack<T, 4>& cv, long long row, bool in) {
+        load_raw<true, false>(xv, static_cast<const T*>(a.x) + row * a.x_stride + c, in);
+        load_raw<true, false>(dv, static_cast<const T*>(a.dt) + row * a.dt_stride + c, in);
+        load_raw<true, false>(zv, static_cast<const T*>(a.z) + row * a.z_stride + c, in && a.z != nullptr);
+        load_raw<VECTOR, false>(bv, static_cast<const T*>(a.bm) + row * a.b_strides[0] + g * a.b_strides[1] + n0, in ? nn : 0);
+        load_raw<VECTOR, false>(cv, static_cast<const T*>(a.cm) + row * a.c_strides[0] + g * a.c_strides[1] + n0, in ? nn : 0);
+    };
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int row = row0 + i;
         slot[i] = row >= a.rows ? -1 : a.slots != nullptr ? a.slots[row] : row;
         if (slot[i] >= a.slot_count) slot[i] = -1;
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
         const bool in = live && slot[i] >= 0;
-        load_f<VECTOR>(h[i], a.state + (in ? slot[i] * a.state_stride + static_cast<long long>(c) * a.dstate + n0 : 0), in ? nn : 0);
+        load_raw<VECTOR, true>(hr[i], a.state + (in ? slot[i] * a.state_stride + static_cast<long long>(c) * a.dstate + n0 : 0),
+                               in ? nn : 0);
+        request(xr[i], dr[i], zr[i], br[i], cr[i], in ? row0 + i : 0, in);
     }
     float a2[4];
     load_f<VECTOR>(a2, a.A + (live ? static_cast<long long>(c) * a.dstate + n0 : 0), live ? nn : 0);
@@ -56,17 +72,15 @@ selective_step_kernel(const SsdScanStepArgs a, int channel_blocks) {
     }
 
     // one token: the state moved on, and its output
-    auto token = [&](float (&s)[4], int row) {
-        float d = 0.f, xv = 0.f;
+    auto token = [&](float (&s)[4], const Pack<T, 1>& xp, const Pack<T, 1>& dp, const Pack<T, 1>& zp, const Pack<T, 4>& bp,
+                     const Pack<T, 4>& cp, int row) {
         float b[4], cv[4];
-        if (live) {
-            d = to_f(static_cast<const T*>(a.dt)[row * a.dt_stride + c]) + bias;
-            xv = to_f(static_cast<const T*>(a.x)[row * a.x_stride + c]);
-        }
+        unpack(b, bp);
+        unpack(cv, cp);
+        const float xv = to_f(xp.v[0]);
+        float d = to_f(dp.v[0]) + bias;
         if (a.softplus) d = softplus_series(d);
         const float u = d * xv;
-        load_f<false>(b, static_cast<const T*>(a.bm) + row * a.b_strides[0] + g * a.b_strides[1] + n0, nn);
-        load_f<false>(cv, static_cast<const T*>(a.cm) + row * a.c_strides[0] + g * a.c_strides[1] + n0, nn);
         float y = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -78,7 +92,7 @@ selective_step_kernel(const SsdScanStepArgs a, int channel_blocks) {
         if (live && part == 0) {
             y = fmaf(skip, xv, y);
             if (a.z != nullptr) {
-                const float zv = to_f(static_cast<const T*>(a.z)[row * a.z_stride + c]);
+                const float zv = to_f(zp.v[0]);
                 y *= zv * sigmoid_fast(zv);
             }
             static_cast<T*>(a.out)[static_cast<long long>(row) * a.channels + c] = from_f<T>(y);
@@ -93,11 +107,18 @@ selective_step_kernel(const SsdScanStepArgs a, int channel_blocks) {
             continue;
         }
         if (found & (1u << i)) continue;  // the first row with this slot takes them all
-        token(h[i], row);
+        float h[4];
+        unpack(h, hr[i]);
+        token(h, xr[i], dr[i], zr[i], br[i], cr[i], row);
         if (found & (0x10000u << i))
             for (int r = row + 1; r < a.rows; ++r)
-                if (a.slots[r] == slot[i]) token(h[i], r);
-        if (live) store_f<VECTOR>(a.state_out + slot[i] * a.state_out_stride + static_cast<long long>(c) * a.dstate + n0, h[i], nn);
+                if (a.slots[r] == slot[i]) {
+                    Pack<T, 1> xv, dv, zv;
+                    Pack<T, 4> bv, cv;
+                    request(xv, dv, zv, bv, cv, r, live);
+                    token(h, xv, dv, zv, bv, cv, r);
+                }
+        if (live) store_f<VECTOR>(a.state_out + slot[i] * a.state_out_stride + static_cast<long long>(c) * a.dstate + n0, h, nn);
     }
 }
 
@@ -115,7 +136,9 @@ extern "C" int ssd_selective_scan_step(const SsdScanStepArgs* args, ssd_stream_t
     if (a.dstate > kScanMaxState) return SSD_ERR_UNSUPPORTED;
     if (!a.x || !a.dt || !a.A || !a.bm || !a.cm || !a.state || !a.state_out || !a.out) return SSD_ERR_NULL;
     const bool vector = a.dstate % 4 == 0 && aligned16(a.A, a.state, a.state_out) && multiple_of(a.state_stride, 4) &&
-                        multiple_of(a.state_out_stride, 4);
+                        multiple_of(a.state_out_stride, 4) && multiple_of(a.b_strides[0] | a.b_strides[1], 4) &&
+                        multiple_of(a.c_strides[0] | a.c_strides[1], 4) &&
+                        aligned_to(a.dtype == SSD_F32 ? 16 : 8, a.bm, a.cm);
     return with_type(a.dtype, [&](auto t) {
         using T = decltype(t);
         const auto launch = [&](auto lpc, auto rows) {

@@ -5,7 +5,7 @@
 //   dpre = dout silu'(pre) ;  din[t] = sum_k w[k] dpre[t + (W-1) - k] ;  dw[k] = sum_t dpre[t] in[t - (W-1) + k]
 //
 // What bounds it: HBM.  A thread owns V neighbouring channels and walks an item of consecutive tokens with the last W
-// inputs in registers, the loads of kAhead tokens in flight; lanes lie along the channels.  An item reads W-1 tokens of
+// inputs in registers, the loads of the next kConvAhead tokens in flight; lanes lie along the channels.  An item reads W-1 tokens of
 // the one before it again (out of L2).
 #include "ssd_vec.cuh"
 
@@ -14,24 +14,42 @@ namespace ssd {
 namespace {
 
 constexpr int kConvThreads = 128;
-constexpr int kConvAhead = 8;
+constexpr int kConvVec = 4;  // channels of a thread: 8 or 16 bytes, a row of filters and inputs in registers for each
+constexpr int kConvAhead = 4;
 
 struct ConvDims {
     SeqMap map;
     int channel_blocks;
 };
 
+// The filters of a CTA's channels, through shared memory: in global memory a channel's taps lie side by side, so that a
+// thread's own loads would touch a line for each of its channels and taps.
 template <class T, int V, int W>
 struct Filter {
+    static constexpr int kChannels = kConvThreads * V, kRow = kChannels + 8;
     float w[W][V], bias[V];
-    __device__ __forceinline__ void load(const SsdConvArgs& a, int c) {
+    __device__ __forceinline__ void load(const void* weight, const void* biases, int f32, int channels, int first) {
+        __shared__ __align__(16) float staged[(W + 1) * kRow];
+        const int n = min(channels - first, kChannels);
+        if (W == 4 && f32 && (reinterpret_cast<uintptr_t>(weight) & 15) == 0) {
+            for (int i = threadIdx.x; i < n; i += kConvThreads) {
+                const float4 t = __ldg(static_cast<const float4*>(weight) + first + i);
+                staged[i] = t.x, staged[kRow + i] = t.y, staged[2 * kRow + i] = t.z, staged[3 * kRow + i] = t.w;
+            }
+        } else {
+            for (int i = threadIdx.x; i < n * W; i += kConvThreads)
+                staged[i % W * kRow + i / W] = load_param<T>(weight, f32, static_cast<long long>(first) * W + i);
+        }
+        for (int i = threadIdx.x; i < n; i += kConvThreads)
+            staged[W * kRow + i] = biases != nullptr ? load_param<T>(biases, f32, first + i) : 0.f;
+        __syncthreads();
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const bool in = c + j < a.channels;
+            const int at = threadIdx.x * V + j;
+            const bool in = at < n;
 #pragma unroll
-            for (int k = 0; k < W; ++k)
-                w[k][j] = in ? load_param<T>(a.weight, a.weight_f32, static_cast<long long>(c + j) * W + k) : 0.f;
-            bias[j] = in && a.bias != nullptr ? load_param<T>(a.bias, a.weight_f32, c + j) : 0.f;
+            for (int k = 0; k < W; ++k) w[k][j] = in ? staged[k * kRow + at] : 0.f;
+            bias[j] = in ? staged[W * kRow + at] : 0.f;
         }
     }
 };
@@ -58,32 +76,39 @@ conv_fwd_kernel(const SsdConvArgs a, const ConvDims d) {
     const int c = (blockIdx.x % d.channel_blocks * kConvThreads + threadIdx.x) * V;
     Span s;
     if (!locate(d.map, item, s)) return;
-    const int n = min(a.channels - c, V);
-    if (n <= 0) return;
+    const int n = max(min(a.channels - c, V), 0);
     T* out = static_cast<T*>(a.out) + ((d.map.cu == nullptr ? s.seq * d.map.tokens : 0) + s.origin) * a.channels + c;
     if (s.pad) {
         const float zero[V] = {};
         for (int t = s.t0; t < s.t1; ++t) store_f<VECTOR>(out + static_cast<long long>(t) * a.channels, zero, n);
         return;
     }
+    const T* x = static_cast<const T*>(a.x) + token_row(d.map, s, a.batch_stride, a.token_stride, 0) + c;
+    Pack<T, V> next[kConvAhead];
+    const auto request = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < kConvAhead; ++i) load_raw<VECTOR, false>(next[i], x + (t + i) * a.token_stride, t + i < s.t1 ? n : 0);
+    };
+    request(s.t0);
     Filter<T, V, W> f;
-    f.load(a, c);
+    f.load(a.weight, a.bias, a.weight_f32, a.channels, c - threadIdx.x * V);
     float held[W][V];  // the last W inputs, held[W-1] the newest
 #pragma unroll
     for (int k = 1; k < W; ++k) load_input<T, V, W, VECTOR>(held[k], a, d.map, s, s.t0 - W + k, c, n);
-    const T* x = static_cast<const T*>(a.x) + token_row(d.map, s, a.batch_stride, a.token_stride, 0) + c;
     for (int t = s.t0; t < s.t1; t += kConvAhead) {
-        float next[kConvAhead][V];
+        Pack<T, V> now[kConvAhead];
 #pragma unroll
-        for (int i = 0; i < kConvAhead; ++i) load_f<VECTOR>(next[i], x + (t + i) * a.token_stride, t + i < s.t1 ? n : 0);
+        for (int i = 0; i < kConvAhead; ++i) now[i] = next[i];
+        if (t + kConvAhead < s.t1) request(t + kConvAhead);
 #pragma unroll
         for (int i = 0; i < kConvAhead; ++i) {
-            float o[V];
+            float o[V], v[V];
+            unpack(v, now[i]);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
 #pragma unroll
                 for (int k = 0; k + 1 < W; ++k) held[k][j] = held[k + 1][j];
-                held[W - 1][j] = next[i][j];
+                held[W - 1][j] = v[j];
                 float p = f.bias[j];
 #pragma unroll
                 for (int k = 0; k < W; ++k) p = fmaf(f.w[k][j], held[k][j], p);
@@ -115,7 +140,7 @@ conv_bwd_kernel(const SsdConvGradArgs g, const ConvDims d, int slices) {
     const int c = (blockIdx.x % d.channel_blocks * kConvThreads + threadIdx.x) * V;
     const int n = max(min(a.channels - c, V), 0);
     Filter<T, V, W> f;
-    f.load(a, c);
+    f.load(a.weight, a.bias, a.weight_f32, a.channels, c - threadIdx.x * V);
     float dw[W][V], db[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -143,17 +168,27 @@ conv_bwd_kernel(const SsdConvGradArgs g, const ConvDims d, int slices) {
 #pragma unroll
             for (int j = 0; j < V; ++j) dpre[k][j] = 0.f;
         }
-        constexpr int kAhead = kConvAhead / 2;
-        for (int t = s.t0; t < s.t1 + W - 1; t += kAhead) {
-            float xs[kAhead][V], ds[kAhead][V];
+        Pack<T, V> xn[kConvAhead], dn[kConvAhead];
+        const int end = min(s.t1 + W - 1, s.len);
+        const auto request = [&](int t) {
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const int in = t + i < s.len && t + i < s.t1 + W - 1 ? n : 0;
-                load_f<VECTOR>(xs[i], x + (t + i) * a.token_stride, in);
-                load_f<VECTOR>(ds[i], dout + static_cast<long long>(t + i) * a.channels, in);
+            for (int i = 0; i < kConvAhead; ++i) {
+                const int in = t + i < end ? n : 0;
+                load_raw<VECTOR, false>(xn[i], x + (t + i) * a.token_stride, in);
+                load_raw<VECTOR, false>(dn[i], dout + static_cast<long long>(t + i) * a.channels, in);
             }
+        };
+        request(s.t0);
+        for (int t = s.t0; t < s.t1 + W - 1; t += kConvAhead) {
+            Pack<T, V> xr[kConvAhead], dr[kConvAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
+            for (int i = 0; i < kConvAhead; ++i) xr[i] = xn[i], dr[i] = dn[i];
+            if (t + kConvAhead < s.t1 + W - 1) request(t + kConvAhead);
+#pragma unroll
+            for (int i = 0; i < kConvAhead; ++i) {
+                float xs[V], ds[V];
+                unpack(xs, xr[i]);
+                unpack(ds, dr[i]);
                 const int to = t + i - (W - 1);  // the input whose gradient is complete with this token
                 const bool mine = t + i < s.t1;
                 float o[V];
@@ -161,8 +196,8 @@ conv_bwd_kernel(const SsdConvGradArgs g, const ConvDims d, int slices) {
                 for (int j = 0; j < V; ++j) {
 #pragma unroll
                     for (int k = 0; k + 1 < W; ++k) held[k][j] = held[k + 1][j], dpre[k][j] = dpre[k + 1][j];
-                    held[W - 1][j] = xs[i][j];
-                    float e = ds[i][j];
+                    held[W - 1][j] = xs[j];
+                    float e = ds[j];
                     if (a.silu) {
                         float p = f.bias[j];
 #pragma unroll
@@ -223,66 +258,82 @@ conv_dw_kernel(const float* table, long long rows, int channels, int width, void
 }
 
 // A generation step: the state and the token in, the state moved on by one and the output out.  A thread owns V channels
-// of a row.  Rows that name the same slot are one another's successors: the first of them does the work of all, each
-// taking the inputs that the one before it left, so that nothing depends on the order of the CTAs.
-template <class T, int V, int W, bool VECTOR>
+// of ROWS rows, whose loads are all in flight together, and their filters.  Rows that name the same slot are one another's
+// successors: the first of them does the work of all, each taking the inputs that the one before it left, so that nothing
+// depends on the order of the CTAs.
+template <class T, int V, int W, int ROWS, bool VECTOR>
 __global__ void __launch_bounds__(kConvThreads)
 conv_step_kernel(const SsdConvStepArgs a, int channel_blocks) {
-    const int row = blockIdx.x / channel_blocks;
+    __shared__ unsigned flags;  // bit i: row i's slot is taken by an earlier row; bit 16 + i: a later row names it too
+    const int row0 = blockIdx.x / channel_blocks * ROWS;
     const int c = (blockIdx.x % channel_blocks * kConvThreads + threadIdx.x) * V;
-    const int n = min(a.channels - c, V);
-    long long slot = row;
-    bool shared = false;
-    if (a.slots != nullptr) {
-        slot = a.slots[row];
-        if (slot < 0 || slot >= a.slot_count) {
-            if (n > 0) {
-                const float zero[V] = {};
-                store_f<VECTOR>(static_cast<T*>(a.out) + static_cast<long long>(row) * a.channels + c, zero, n);
-            }
-            return;
-        }
-        bool before = false, after = false;
-        for (int r = threadIdx.x; r < a.rows; r += kConvThreads) {
-            const bool same = a.slots[r] == slot;
-            before |= same && r < row;
-            after |= same && r > row;
-        }
-        if (__syncthreads_or(before)) return;
-        shared = __syncthreads_or(after);
-    }
-    if (n <= 0) return;
-    const SsdConvArgs filter{nullptr, a.weight, a.bias, nullptr, nullptr, nullptr, nullptr, 0, 0, 0, 0, a.channels, W, a.dtype,
-                             a.weight_f32, a.silu};
-    float held[W][V];
-    const T* state = static_cast<const T*>(a.state) + slot * a.state_stride + c;
+    const int n = max(min(a.channels - c, V), 0);
+    long long slot[ROWS];
 #pragma unroll
-    for (int k = 1; k < W; ++k) load_f<VECTOR>(held[k], state + static_cast<long long>(k - 1) * a.channels, n);
+    for (int i = 0; i < ROWS; ++i) {
+        const int row = row0 + i;
+        slot[i] = row >= a.rows ? -1 : a.slots != nullptr ? a.slots[row] : row;
+        if (slot[i] >= a.slot_count) slot[i] = -1;
+    }
+    Pack<T, V> raw[ROWS][W];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int in = slot[i] >= 0 ? n : 0;
+        const T* state = static_cast<const T*>(a.state) + (in ? slot[i] * a.state_stride + c : 0);
+#pragma unroll
+        for (int k = 0; k + 1 < W; ++k) load_raw<VECTOR, true>(raw[i][k], state + static_cast<long long>(k) * a.channels, in);
+        load_raw<VECTOR, false>(raw[i][W - 1], static_cast<const T*>(a.x) + (in ? (row0 + i) * a.x_stride + c : 0), in);
+    }
+    if (threadIdx.x == 0) flags = 0;
     Filter<T, V, W> f;
-    f.load(filter, c);
-    int r = row;
-    while (true) {
-        float x[V], o[V];
-        load_f<VECTOR>(x, static_cast<const T*>(a.x) + r * a.x_stride + c, n);
+    f.load(a.weight, a.bias, a.weight_f32, a.channels, c - threadIdx.x * V);
+    unsigned found = 0;
+    if (a.slots != nullptr) {
+        unsigned bits = 0;
+        for (int r = threadIdx.x; r < a.rows; r += kConvThreads) {
+            const int other = a.slots[r];
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i)
+                if (other == slot[i] && r != row0 + i) bits |= r < row0 + i ? 1u << i : 0x10000u << i;
+        }
+        if (bits != 0) atomicOr(&flags, bits);
+        __syncthreads();
+        found = flags;
+    }
+    auto token = [&](const Pack<T, V> (&held)[W], int row) {
+        float o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-#pragma unroll
-            for (int k = 0; k + 1 < W; ++k) held[k][j] = held[k + 1][j];
-            held[W - 1][j] = x[j];
             float p = f.bias[j];
 #pragma unroll
-            for (int k = 0; k < W; ++k) p = fmaf(f.w[k][j], held[k][j], p);
+            for (int k = 0; k < W; ++k) p = fmaf(f.w[k][j], to_f(held[k].v[j]), p);
             o[j] = a.silu ? p * sigmoid_fast(p) : p;
         }
-        store_f<VECTOR>(static_cast<T*>(a.out) + static_cast<long long>(r) * a.channels + c, o, n);
-        if (!shared) break;
-        do ++r;
-        while (r < a.rows && a.slots[r] != slot);
-        if (r >= a.rows) break;
-    }
-    T* next = static_cast<T*>(a.state_out) + slot * a.state_out_stride + c;
+        store_f<VECTOR>(static_cast<T*>(a.out) + static_cast<long long>(row) * a.channels + c, o, n);
+    };
 #pragma unroll
-    for (int k = 1; k < W; ++k) store_f<VECTOR>(next + static_cast<long long>(k - 1) * a.channels, held[k], n);
+    for (int i = 0; i < ROWS; ++i) {
+        const int row = row0 + i;
+        if (row >= a.rows) break;
+        if (slot[i] < 0) {
+            const float zero[V] = {};
+            store_f<VECTOR>(static_cast<T*>(a.out) + static_cast<long long>(row) * a.channels + c, zero, n);
+            continue;
+        }
+        if (found & (1u << i)) continue;  // the first row with this slot takes them all
+        token(raw[i], row);
+        if (found & (0x10000u << i))
+            for (int r = row + 1; r < a.rows; ++r)
+                if (a.slots[r] == slot[i]) {
+#pragma unroll
+                    for (int k = 0; k + 1 < W; ++k) raw[i][k] = raw[i][k + 1];
+                    load_raw<VECTOR, false>(raw[i][W - 1], static_cast<const T*>(a.x) + r * a.x_stride + c, n);
+                    token(raw[i], r);
+                }
+        T* next = static_cast<T*>(a.state_out) + slot[i] * a.state_out_stride + c;
+#pragma unroll
+        for (int k = 1; k < W; ++k) store_raw<VECTOR>(next + static_cast<long long>(k - 1) * a.channels, raw[i][k], n);
+    }
 }
 
 int conv_check(const SsdConvArgs& a) {
@@ -302,23 +353,27 @@ int with_width(int width, F f) {
         default: return f(std::integral_constant<int, 4>{});
     }
 }
-// Tokens of an item: as many as leave about eight CTAs per SM, so that little is read twice.
-int conv_span(const SsdConvArgs& a, int channel_blocks, int least, int most) {
+// Tokens of an item of the forward pass: as many as leave about six CTAs per SM, so that little is read twice.
+int conv_span(const SsdConvArgs& a, int channel_blocks) {
     const long long total = a.cu_seqlens ? a.tokens : a.tokens * a.rows;
-    int span = most;
-    while (span > least && total / span * channel_blocks < 8LL * sm_count()) span /= 2;
+    int span = 64;
+    while (span > 8 && total / span * channel_blocks < 6LL * sm_count()) span /= 2;
     return span;
 }
-template <class T>
-constexpr int kConvVec = 16 / static_cast<int>(sizeof(T));  // forward and step: 16 bytes
-constexpr int kConvGradVec = 4;                              // four rows of W registers per channel: 8 or 16 bytes
-ConvDims conv_grad_dims(const SsdConvArgs& a) {
-    const int blocks = (a.channels + kConvThreads * kConvGradVec - 1) / (kConvThreads * kConvGradVec);
-    return ConvDims{{a.cu_seqlens, a.tokens, a.rows, conv_span(a, blocks, 16, 128)}, blocks};
+// Backward, the CTAs that the SMs hold at a time (three each, by registers) are dealt one item each where the sequences allow.
+constexpr int kConvGradCtas = 3;
+long long conv_grad_slices(int channel_blocks) {
+    return (static_cast<long long>(kConvGradCtas) * sm_count() + channel_blocks - 1) / channel_blocks;
 }
-// CTAs per channel block: what the SMs hold at a time (four of them each, by registers).
+ConvDims conv_grad_dims(const SsdConvArgs& a) {
+    const int blocks = (a.channels + kConvThreads * kConvVec - 1) / (kConvThreads * kConvVec);
+    const long long slices = conv_grad_slices(blocks), sequences = a.cu_seqlens ? 1 : a.rows;
+    const long long per = slices > sequences ? slices / sequences : 1;
+    const long long span = (a.tokens + per - 1) / per;
+    return ConvDims{{a.cu_seqlens, a.tokens, a.rows, static_cast<int>(span < 16 ? 16 : span)}, blocks};
+}
 int conv_slices(const ConvDims& d) {
-    const long long items = d.map.items(), fill = (4LL * sm_count() + d.channel_blocks - 1) / d.channel_blocks;
+    const long long items = d.map.items(), fill = conv_grad_slices(d.channel_blocks);
     return static_cast<int>(items < fill ? items : fill);
 }
 
@@ -334,12 +389,12 @@ extern "C" int ssd_short_conv_fwd(const SsdConvArgs* args, ssd_stream_t stream) 
     if (!a.out && a.tokens > 0) return SSD_ERR_NULL;
     return with_type(a.dtype, [&](auto t) {
         using T = decltype(t);
-        constexpr int V = kConvVec<T>;
+        constexpr int V = kConvVec;
         const int channel_blocks = (a.channels + kConvThreads * V - 1) / (kConvThreads * V);
-        const ConvDims d{{a.cu_seqlens, a.tokens, a.rows, conv_span(a, channel_blocks, 8, 32)}, channel_blocks};
+        const ConvDims d{{a.cu_seqlens, a.tokens, a.rows, conv_span(a, channel_blocks)}, channel_blocks};
         const long long blocks = d.map.items() * channel_blocks;
         if (blocks > 0x7fffffffLL) return static_cast<int>(SSD_ERR_RANGE);
-        const bool vector = aligned16(a.x, a.initial_state, a.out, a.final_state) && multiple_of(a.channels, V) &&
+        const bool vector = aligned_to(sizeof(T) * V, a.x, a.initial_state, a.out, a.final_state) && multiple_of(a.channels, V) &&
                             multiple_of(a.batch_stride, V) && multiple_of(a.token_stride, V);
         return with_width(a.width, [&](auto w) {
             constexpr int W = decltype(w)::value;
@@ -370,7 +425,7 @@ extern "C" int ssd_short_conv_bwd(const SsdConvGradArgs* args, ssd_stream_t stre
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return with_type(a.dtype, [&](auto t) {
         using T = decltype(t);
-        constexpr int V = kConvGradVec;
+        constexpr int V = kConvVec;
         const bool vector = aligned_to(sizeof(T) * V, a.x, a.initial_state, g.dout, g.dfinal, g.dx, g.dinitial) &&
                             multiple_of(a.channels, V) && multiple_of(a.batch_stride, V) && multiple_of(a.token_stride, V);
         const int rc = with_width(a.width, [&](auto w) {
@@ -398,16 +453,24 @@ extern "C" int ssd_short_conv_step(const SsdConvStepArgs* args, ssd_stream_t str
     if (!a.x || !a.weight || !a.state || !a.state_out || !a.out) return SSD_ERR_NULL;
     return with_type(a.dtype, [&](auto t) {
         using T = decltype(t);
-        constexpr int V = kConvVec<T>;
+        constexpr int V = kConvVec;
         const int channel_blocks = (a.channels + kConvThreads * V - 1) / (kConvThreads * V);
-        const long long blocks = static_cast<long long>(a.rows) * channel_blocks;
+        // several rows share the filters; one where that would leave SMs without a CTA
+        const int rows = static_cast<long long>(a.rows) * channel_blocks >= 8LL * sm_count() ? 4 : 1;
+        const long long blocks = static_cast<long long>((a.rows + rows - 1) / rows) * channel_blocks;
         if (blocks > 0x7fffffffLL) return static_cast<int>(SSD_ERR_RANGE);
-        const bool vector = aligned16(a.x, a.state, a.state_out, a.out) && multiple_of(a.channels, V) &&
+        const bool vector = aligned_to(sizeof(T) * V, a.x, a.state, a.state_out, a.out) && multiple_of(a.channels, V) &&
                             multiple_of(a.x_stride, V) && multiple_of(a.state_stride, V) && multiple_of(a.state_out_stride, V);
         return with_width(a.width, [&](auto w) {
             constexpr int W = decltype(w)::value;
-            launch_plain(vector ? conv_step_kernel<T, V, W, true> : conv_step_kernel<T, V, W, false>,
-                         static_cast<unsigned>(blocks), kConvThreads, 0, reinterpret_cast<cudaStream_t>(stream), a, channel_blocks);
+            const auto launch = [&](auto kernel) {
+                launch_plain(kernel, static_cast<unsigned>(blocks), kConvThreads, 0, reinterpret_cast<cudaStream_t>(stream), a,
+                             channel_blocks);
+            };
+            if (rows > 1)
+                vector ? launch(conv_step_kernel<T, V, W, 4, true>) : launch(conv_step_kernel<T, V, W, 4, false>);
+            else
+                vector ? launch(conv_step_kernel<T, V, W, 1, true>) : launch(conv_step_kernel<T, V, W, 1, false>);
             return launch_status();
         });
     });

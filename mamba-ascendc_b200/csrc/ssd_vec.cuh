@@ -33,48 +33,58 @@ struct Bits<8> { using type = uint2; };
 template <>
 struct Bits<16> { using type = uint4; };
 
-// V elements as they lie in memory; V * sizeof(T) is 4, 8, 16 or a multiple of 16.
+// V elements as they lie in memory; V * sizeof(T) is 2, 4, 8, 16 or a multiple of 16.
 template <class T, int V>
 struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) * V) Pack {
     T v[V];
 };
 
-// V elements from p, n of them in range (the rest zero).  VECTOR: p is aligned for the whole vector and n is 0 or V.
+// V elements from p, n of them in range (the rest zero), not yet converted: a load that is to be in flight under other work
+// must not be followed by its conversion, at which the warp would wait.  VECTOR: p is aligned for the whole vector and n is
+// 0 or V.  KEPT: the memory is written by this kernel as well; otherwise the read may pass stores.
+template <bool VECTOR, bool KEPT, int V, class T>
+__device__ __forceinline__ void load_raw(Pack<T, V>& raw, const T* p, int n) {
+    constexpr int kStep = VECTOR ? (sizeof(raw) < 16 ? sizeof(raw) : 16) : sizeof(T), kLoads = sizeof(raw) / kStep;
+    using B = typename Bits<kStep>::type;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        B v{};
+        if (VECTOR ? n > 0 : i < n) v = KEPT ? reinterpret_cast<const B*>(p)[i] : __ldg(reinterpret_cast<const B*>(p) + i);
+        reinterpret_cast<B*>(&raw)[i] = v;
+    }
+}
+template <int V, class T>
+__device__ __forceinline__ void unpack(float (&f)[V], const Pack<T, V>& raw) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = to_f(raw.v[i]);
+}
 template <bool VECTOR, int V, class T>
 __device__ __forceinline__ void load_f(float (&f)[V], const T* p, int n) {
-    if constexpr (VECTOR) {
-        Pack<T, V> raw;
-        if (n > 0) {
-            constexpr int kStep = sizeof(raw) < 16 ? sizeof(raw) : 16;
-            using B = typename Bits<kStep>::type;
+    Pack<T, V> raw;
+    load_raw<VECTOR, false>(raw, p, n);
+    unpack(f, raw);
+}
+// of memory that this kernel writes as well
+template <bool VECTOR, int V, class T>
+__device__ __forceinline__ void load_kept(float (&f)[V], const T* p, int n) {
+    Pack<T, V> raw;
+    load_raw<VECTOR, true>(raw, p, n);
+    unpack(f, raw);
+}
+template <bool VECTOR, int V, class T>
+__device__ __forceinline__ void store_raw(T* p, const Pack<T, V>& raw, int n) {
+    constexpr int kStep = VECTOR ? (sizeof(raw) < 16 ? sizeof(raw) : 16) : sizeof(T), kStores = sizeof(raw) / kStep;
+    using B = typename Bits<kStep>::type;
 #pragma unroll
-            for (int i = 0; i < static_cast<int>(sizeof(raw)) / kStep; ++i)
-                reinterpret_cast<B*>(&raw)[i] = reinterpret_cast<const B*>(p)[i];
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = n > 0 ? to_f(raw.v[i]) : 0.f;
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = i < n ? to_f(p[i]) : 0.f;
-    }
+    for (int i = 0; i < kStores; ++i)
+        if (VECTOR ? n > 0 : i < n) reinterpret_cast<B*>(p)[i] = reinterpret_cast<const B*>(&raw)[i];
 }
 template <bool VECTOR, int V, class T>
 __device__ __forceinline__ void store_f(T* p, const float (&f)[V], int n) {
-    if constexpr (VECTOR) {
-        if (n <= 0) return;
-        Pack<T, V> raw;
+    Pack<T, V> raw;
 #pragma unroll
-        for (int i = 0; i < V; ++i) raw.v[i] = from_f<T>(f[i]);
-        constexpr int kStep = sizeof(raw) < 16 ? sizeof(raw) : 16;
-        using B = typename Bits<kStep>::type;
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(raw)) / kStep; ++i)
-            reinterpret_cast<B*>(p)[i] = reinterpret_cast<const B*>(&raw)[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < n) p[i] = from_f<T>(f[i]);
-    }
+    for (int i = 0; i < V; ++i) raw.v[i] = from_f<T>(f[i]);
+    store_raw<VECTOR>(p, raw, n);
 }
 
 // Parameters come in fp32 or in the activations' type, by a flag that is the same for every thread.
