@@ -172,7 +172,7 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
 
         F2 ddt2[kTokens], du[kTokens], y[kTokens];
 #pragma unroll
-        for (int i = 0; i < kTokens; ++i) ddt2[i] = du[i] = y[i] = 0;
+        for (int i = 0; i < kTokens; ++i) ddt2[i] = du[i] = y[i] = {};
         const F2 total_dt = pack2(sum_dt.x, sum_dt.y);
         const float* hp = a.checkpoints + (checkpoint0 + t0 / kScanCheckpoint) * N * a.channels + c;
         if (k > 0 && lane < kTokens) {  // the next chunk's rows (the tokens before) into L2
@@ -196,7 +196,7 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
                 *reinterpret_cast<float4*>(ct + i) = *reinterpret_cast<const float4*>(sc + n * kRow + w * kTokens + i);
             }
             F2 al[kTokens], h[kTokens];
-            F2 end_h = 0, end_g = 0;
+            F2 end_h = {}, end_g = {};
 #pragma unroll
             for (int i = 0; i < kTokens; ++i) {
                 al[i] = exp2_2(mul2(dt[i], a2));
@@ -252,7 +252,7 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
                     if (GATED) y[i] = fma2(pack2(ct[i], ct[i]), prev, y[i]);
                 }
             }
-            F2 da = 0;
+            F2 da = {};
 #pragma unroll
             for (int i = kTokens - 1; i >= 0; --i) {
                 const F2 gt = fma2(pack2(ct[i], ct[i]), dy[i], gs);

@@ -2,14 +2,15 @@
 //
 //   a_t[n] = exp(dt_t A[n]) ;  h_t[n] = a_t[n] h_{t-1}[n] + dt_t x_t B_t[n] ;  y_t = sum_n C_t[n] h_t[n]   for every channel
 //
-// What bounds it: one exponential and two multiply-adds with two products for each (token, channel, state column), not the
-// bytes (with 16 columns 16 exponentials for 8 bytes).  An SM forms 16 exponentials a cycle, eight cycles for a warp's.
-// The walk over the tokens is serial with the state in registers, so that each exponential is formed once.
+// What bounds it: instructions.  Each (token, channel, state column) takes an exponential (an SM forms 16 a cycle, eight cycles
+// for a warp's), two products and two multiply-adds, each (token, channel) about 45 more for softplus, gate, loads and stores,
+// while with 16 columns the bytes are 8 for 16 exponentials.  The walk over the tokens is serial with the state in registers,
+// so that each exponential is formed once.
 //
-// Layout: a lane owns a channel, a warp NPL state columns of 32 channels, NW warps all columns of them, a CTA `cg` such sets.
-// B and C are the same for all lanes (one broadcast load for four columns), and nothing is exchanged between lanes; the NW
+// Layout: a lane owns a channel, a warp NPL state columns of 32 channels, the NW warps of a CTA all columns of them.  B and C
+// are the same for all lanes (one broadcast load for two tokens of a column), and nothing is exchanged between lanes; the NW
 // partial sums of y meet in shared memory.  Tokens pass through shared memory kScanTile at a time: dt (softplus taken once)
-// and dt x as pairs, B and C in fp32.  The next tile's loads are in flight under the walk.
+// and dt x of two tokens side by side, B and C in fp32.  The next tile's loads are in flight under the walk.
 //
 // kMode: the forward pass itself; each segment's end state from a zero start; or backward in time, the gradient that a segment
 // hands to the state before it, e <- a_t (e + C_t dy_t), with dy = dout silu(z).
@@ -22,255 +23,261 @@ namespace ssd {
 namespace {
 
 constexpr int kScanTile = 32;
+constexpr int kTileRow = kScanTile + 4;  // tokens of a column in shared memory, padded
+constexpr int kWalkChannels = 32;
 enum ScanMode { kForward, kEndState, kStartGradient };
 
 struct ScanLaunch {
     SeqMap map;
     ScanBlocks blocks;
-    int cg;
     bool split;            // start states come from `work`
     float* work;           // [items][dstate][channels], [items][channels]
     const void* dout;      // kStartGradient
 };
 
+template <int NPL, int NW, ScanMode kMode>
+struct WalkSmem {
+    static constexpr int kCols = NPL * NW;  // state columns, those behind dstate are zeros
+    float4 du[kScanTile / 2][kWalkChannels];  // dt of two tokens, dt x (or dy) of them
+    float b[kCols][kTileRow];                 // B, or C
+    float c[kMode == kForward ? kCols : 1][kTileRow];
+    float2 y[kMode == kForward ? NW : 1][kScanTile / 2][kWalkChannels];
+};
+
 template <class T, int NPL, int NW, bool VECTOR, ScanMode kMode>
-__global__ void __launch_bounds__(32 * NW * (NW >= 8 ? 1 : 8 / NW))
+__global__ void __launch_bounds__(32 * NW)
 selective_walk_kernel(const SsdScanArgs a, const ScanLaunch l) {
-    constexpr int kCols = NPL * NW;               // state columns, those behind dstate are zeros
-    constexpr int kPairs = kScanTile / (2 * NW);  // channel pairs of a tile that a thread stages
-    constexpr int kShared = 2 * NPL;              // B and C elements that a thread stages (with one channel set)
+    using Smem = WalkSmem<NPL, NW, kMode>;
+    constexpr int kCols = Smem::kCols, kThreads = 32 * NW;
     constexpr bool kReverse = kMode == kStartGradient;
-    extern __shared__ __align__(16) float walk_smem[];
+    extern __shared__ __align__(16) unsigned char walk_smem[];
+    Smem& sm = *reinterpret_cast<Smem*>(walk_smem);
     const int blocks = l.blocks.count(a.groups);
     const long long item = blockIdx.x / blocks;
     const ChannelBlock cb = channel_block(l.blocks, blockIdx.x % blocks, a.channels, a.groups);
     Span s;
     if (!locate(l.map, item, s)) return;
-    const int tid = threadIdx.x, threads = 32 * NW * l.cg, lane = tid & 31, warp = tid >> 5;
-    const int channels_here = 32 * l.cg, row_pairs = 16 * l.cg;  // a power of two
-    const long long rows_before = l.map.cu == nullptr ? s.seq * l.map.tokens : 0;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long first_token = (l.map.cu == nullptr ? s.seq * l.map.tokens : 0) + s.origin;
 
     if (s.pad) {
         if (kMode == kForward)
-            for (long long i = tid; i < static_cast<long long>(s.t1 - s.t0) * cb.n; i += threads) {
-                const long long t = i / cb.n;
-                static_cast<T*>(a.out)[(s.origin + s.t0 + t) * a.channels + cb.first + i % cb.n] = from_f<T>(0.f);
-            }
+            for (long long i = tid; i < static_cast<long long>(s.t1 - s.t0) * cb.n; i += kThreads)
+                static_cast<T*>(a.out)[(s.origin + s.t0 + i / cb.n) * a.channels + cb.first + i % cb.n] = from_f<T>(0.f);
         return;
     }
 
-    float2* sdu = reinterpret_cast<float2*>(walk_smem);       // [tile][channels] dt, dt x (or dy)
-    float* sb = walk_smem + 2 * kScanTile * channels_here;    // [tile][kCols] B (or C)
-    float* sc = sb + kScanTile * kCols;                       // [tile][kCols]
-    float* sy = sc + kScanTile * kCols;                       // [NW][tile][channels]
-
     // ---- the walk's own state
-    const int wn = warp % NW, wc = warp / NW;
-    const int mine = wc * 32 + lane, c = cb.first + mine, n0 = wn * NPL;
-    const bool live = mine < cb.n;
-    F2 h[NPL / 2], a2[NPL / 2];
+    const int c = cb.first + lane, n0 = warp * NPL;
+    const bool live = lane < cb.n;
+    float h[NPL], a2[NPL];
     float sum_dt = 0.f;
-    const float* start = l.work + item * a.dstate * a.channels;
 #pragma unroll
-    for (int j = 0; j < NPL; j += 2) {
-        float av[2], hv[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int n = n0 + j + i;
-            const bool in = live && n < a.dstate;
-            av[i] = in ? a.A[static_cast<long long>(c) * a.dstate + n] * kLog2e : 0.f;
-            hv[i] = 0.f;
-            if (kMode == kForward && in) {
-                if (l.split)
-                    hv[i] = start[static_cast<long long>(n) * a.channels + c];
-                else if (a.initial_state != nullptr)
-                    hv[i] = a.initial_state[(static_cast<long long>(s.seq) * a.channels + c) * a.dstate + n];
-            }
+    for (int j = 0; j < NPL; ++j) {
+        const int n = n0 + j;
+        const bool in = live && n < a.dstate;
+        a2[j] = in ? a.A[static_cast<long long>(c) * a.dstate + n] * kLog2e : 0.f;
+        h[j] = 0.f;
+        if (kMode == kForward && in) {
+            if (l.split)
+                h[j] = l.work[(item * a.dstate + n) * a.channels + c];
+            else if (a.initial_state != nullptr)
+                h[j] = a.initial_state[(static_cast<long long>(s.seq) * a.channels + c) * a.dstate + n];
         }
-        a2[j / 2] = pack2(av[0], av[1]);
-        h[j / 2] = pack2(hv[0], hv[1]);
     }
+    const long long checkpoint0 = l.map.cu == nullptr
+                                      ? s.seq * ((l.map.tokens + kScanCheckpoint - 1) / kScanCheckpoint)
+                                      : s.origin / kScanCheckpoint + s.seq;
 
-    // ---- staging
-    const T* x = static_cast<const T*>(a.x) + token_row(l.map, s, a.x_strides[0], a.x_strides[1], 0) + cb.first;
-    const T* dt = static_cast<const T*>(a.dt) + token_row(l.map, s, a.dt_strides[0], a.dt_strides[1], 0) + cb.first;
-    const T* z = static_cast<const T*>(a.z) + token_row(l.map, s, a.z_strides[0], a.z_strides[1], 0) + cb.first;
-    const T* bm = static_cast<const T*>(kReverse ? a.cm : a.bm) +
-                  token_row(l.map, s, kReverse ? a.c_strides[0] : a.b_strides[0], kReverse ? a.c_strides[1] : a.b_strides[1], 0) +
-                  cb.group * (kReverse ? a.c_strides[2] : a.b_strides[2]);
-    const int64_t b_step = kReverse ? a.c_strides[1] : a.b_strides[1];
-    const T* cm = static_cast<const T*>(a.cm) + token_row(l.map, s, a.c_strides[0], a.c_strides[1], 0) +
-                  cb.group * a.c_strides[2];
-    T* out = static_cast<T*>(a.out) + (rows_before + s.origin) * a.channels + cb.first;
-    const T* dout = static_cast<const T*>(l.dout) + (rows_before + s.origin) * a.channels + cb.first;
-    const int pair = tid & (row_pairs - 1), first_row = tid / row_pairs, row_step = threads / row_pairs;  // 2 NW rows a step
-    const int pn = min(cb.n - 2 * pair, 2);
+    // ---- staging: a thread has two neighbouring channels of kPairs tokens, two neighbouring ones at a time, and quads of
+    // state columns of B and C
+    constexpr int kPairs = 16 / NW, kQuads = NPL / 2, kArrayQuads = kScanTile * kCols / 4;
+    const int pair = tid & 15, pn = max(min(cb.n - 2 * pair, 2), 0), c2 = cb.first + 2 * pair;
+    const auto row_at = [&](int p) { return 2 * ((tid >> 4) + p / 2 * 2 * NW) + p % 2; };
     float2 bias = make_float2(0.f, 0.f), skip = bias;
-    if (pn > 0) {
-        if (a.dt_bias != nullptr)
-            bias = make_float2(a.dt_bias[cb.first + 2 * pair], pn > 1 ? a.dt_bias[cb.first + 2 * pair + 1] : 0.f);
-        if (a.D != nullptr) skip = make_float2(a.D[cb.first + 2 * pair], pn > 1 ? a.D[cb.first + 2 * pair + 1] : 0.f);
-    }
-    const int shared_each = kShared / l.cg;  // of them
+    if (a.dt_bias != nullptr) bias = make_float2(pn > 0 ? a.dt_bias[c2] : 0.f, pn > 1 ? a.dt_bias[c2 + 1] : 0.f);
+    if (a.D != nullptr) skip = make_float2(pn > 0 ? a.D[c2] : 0.f, pn > 1 ? a.D[c2 + 1] : 0.f);
+    const Rows<T> xs = kReverse ? Rows<T>(static_cast<const T*>(l.dout) + first_token * a.channels + c2, a.channels)
+                                : Rows<T>(static_cast<const T*>(a.x) + first_row(l.map, s, a.x_strides) + c2, a.x_strides[1]);
+    const Rows<T> dts(static_cast<const T*>(a.dt) + first_row(l.map, s, a.dt_strides) + c2, a.dt_strides[1]);
+    const Rows<T> zs(static_cast<const T*>(a.z) + first_row(l.map, s, a.z_strides) + c2, a.z_strides[1]);
+    const Rows<T> bs(static_cast<const T*>(a.bm) + first_row(l.map, s, a.b_strides) + cb.group * a.b_strides[2], a.b_strides[1]);
+    const Rows<T> cs(static_cast<const T*>(a.cm) + first_row(l.map, s, a.c_strides) + cb.group * a.c_strides[2], a.c_strides[1]);
+    T* out = static_cast<T*>(a.out) + first_token * a.channels + c2;
+
     Pack<T, 2> xr[kPairs], dr[kPairs], zr[kPairs];
-    Pack<T, 1> br[kShared];
-    auto request = [&](int t0) {
+    Pack<T, 4> qr[kQuads];
+    // quad i of this thread: of B in the first half of their numbers, of C in the second (backwards C takes B's place)
+    const auto quad_of_c = [&](int i) { return kReverse || tid + i * kThreads >= kArrayQuads; };
+    const auto has_quad = [&](int i) { return kMode == kForward || tid + i * kThreads < kArrayQuads; };
+    const auto quad_row = [&](int i) { return (tid + i * kThreads) % kArrayQuads / (kCols / 4); };
+    const auto quad_col = [&](int i) { return (tid + i * kThreads) % (kCols / 4) * 4; };
+    const auto request = [&](int t0) {
 #pragma unroll
         for (int p = 0; p < kPairs; ++p) {
-            const int t = t0 + first_row + p * row_step;
-            const int n = t < s.t1 ? pn : 0;
-            load_raw<VECTOR, false>(dr[p], dt + t * a.dt_strides[1] + 2 * pair, n);
-            if (kReverse) {
-                load_raw<VECTOR, false>(xr[p], dout + static_cast<long long>(t) * a.channels + 2 * pair, n);
-                if (a.z != nullptr) load_raw<VECTOR, false>(zr[p], z + t * a.z_strides[1] + 2 * pair, n);
-            } else {
-                load_raw<VECTOR, false>(xr[p], x + t * a.x_strides[1] + 2 * pair, n);
-            }
+            const int t = t0 + row_at(p), n = t < s.t1 ? pn : 0;
+            load_raw<VECTOR, false>(xr[p], xs.at(t), n);
+            load_raw<VECTOR, false>(dr[p], dts.at(t), n);
+            if (kReverse && a.z != nullptr) load_raw<VECTOR, false>(zr[p], zs.at(t), n);
         }
 #pragma unroll
-        for (int p = 0; p < kShared; ++p) {
-            const int i = tid + (p / 2) * threads, t = t0 + i / kCols, n = i % kCols;
-            const int in = p < shared_each && n < a.dstate && t < s.t1 ? 1 : 0;
-            if (p % 2 == 0)
-                load_raw<true, false>(br[p], bm + t * b_step + n, in);
-            else if (kMode == kForward)
-                load_raw<true, false>(br[p], cm + t * a.c_strides[1] + n, in);
-        }
+        for (int i = 0; i < kQuads; ++i)
+            if (has_quad(i)) {
+                const int t = t0 + quad_row(i), n = quad_col(i);
+                load_raw<VECTOR, false>(qr[i], (quad_of_c(i) ? cs : bs).at(t) + n, t < s.t1 ? min(a.dstate - n, 4) : 0);
+            }
     };
     const int tiles = (s.t1 - s.t0 + kScanTile - 1) / kScanTile;
-    auto tile_start = [&](int k) { return s.t0 + (kReverse ? tiles - 1 - k : k) * kScanTile; };
+    const auto tile_start = [&](int k) { return s.t0 + (kReverse ? tiles - 1 - k : k) * kScanTile; };
     if (tiles > 0) request(tile_start(0));
 
     for (int k = 0; k < tiles; ++k) {
         const int t0 = tile_start(k), nt = min(s.t1 - t0, kScanTile);
         float2 held[kPairs];  // x, for the skip connection
 #pragma unroll
-        for (int p = 0; p < kPairs; ++p) {
-            const int row = first_row + p * row_step;
-            const bool in = row < nt;
-            const float2 xv = pair_f(xr[p]);
-            float2 d = pair_f(dr[p]);
-            d = make_float2(d.x + bias.x, d.y + bias.y);
-            if (a.softplus) d = make_float2(softplus_series(d.x), softplus_series(d.y));
-            if (!in) d = make_float2(0.f, 0.f);  // behind the last token the state stays
-            float2 u;
-            if (kReverse) {
-                u = xv;
-                if (a.z != nullptr) {
-                    const float2 zv = pair_f(zr[p]);
-                    u = make_float2(u.x * zv.x * sigmoid_fast(zv.x), u.y * zv.y * sigmoid_fast(zv.y));
+        for (int p = 0; p < kPairs; p += 2) {
+            float2 d[2], u[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float2 xv = pair_f(xr[p + i]);
+                d[i] = pair_f(dr[p + i]);
+                d[i] = make_float2(d[i].x + bias.x, d[i].y + bias.y);
+                if (a.softplus) d[i] = make_float2(softplus_series(d[i].x), softplus_series(d[i].y));
+                if (row_at(p + i) >= nt) d[i] = make_float2(0.f, 0.f);  // behind the last token the state stays
+                if (kReverse) {
+                    u[i] = xv;
+                    if (a.z != nullptr) {
+                        const float2 zv = pair_f(zr[p + i]);
+                        u[i] = make_float2(xv.x * zv.x * sigmoid_fast(zv.x), xv.y * zv.y * sigmoid_fast(zv.y));
+                    }
+                } else {
+                    u[i] = make_float2(d[i].x * xv.x, d[i].y * xv.y);
                 }
-            } else {
-                u = make_float2(d.x * xv.x, d.y * xv.y);
+                held[p + i] = xv;
             }
-            held[p] = xv;
-            *reinterpret_cast<float4*>(&sdu[row * channels_here + 2 * pair]) = make_float4(d.x, u.x, d.y, u.y);
+            float4* at = &sm.du[row_at(p) / 2][2 * pair];
+            at[0] = make_float4(d[0].x, d[1].x, u[0].x, u[1].x);
+            at[1] = make_float4(d[0].y, d[1].y, u[0].y, u[1].y);
         }
 #pragma unroll
-        for (int p = 0; p < kShared; ++p)
-            if (p < shared_each && (p % 2 == 0 || kMode == kForward))
-                (p % 2 == 0 ? sb : sc)[tid + (p / 2) * threads] = to_f(br[p].v[0]);
+        for (int i = 0; i < kQuads; ++i)
+            if (has_quad(i)) {
+                float* dst = (kMode == kForward && quad_of_c(i) ? sm.c : sm.b)[quad_col(i)] + quad_row(i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dst[j * kTileRow] = to_f(qr[i].v[j]);
+            }
         __syncthreads();
         if (k + 1 < tiles) request(tile_start(k + 1));
         if (kMode == kForward && a.z != nullptr) {
 #pragma unroll
-            for (int p = 0; p < kPairs; ++p) {
-                const int t = t0 + first_row + p * row_step;
-                load_raw<VECTOR, false>(zr[p], z + t * a.z_strides[1] + 2 * pair, t < s.t1 ? pn : 0);
-            }
+            for (int p = 0; p < kPairs; ++p)
+                load_raw<VECTOR, false>(zr[p], zs.at(t0 + row_at(p)), row_at(p) < nt ? pn : 0);
         }
         if (kMode == kForward && a.checkpoints != nullptr && (t0 - s.t0) % kScanCheckpoint == 0 && live) {
-            const long long at = (l.map.cu == nullptr ? s.seq * ((l.map.tokens + kScanCheckpoint - 1) / kScanCheckpoint)
-                                                      : s.origin / kScanCheckpoint + s.seq) + t0 / kScanCheckpoint;
-            float* dst = a.checkpoints + at * a.dstate * a.channels + c;
+            float* dst = a.checkpoints + (checkpoint0 + t0 / kScanCheckpoint) * a.dstate * a.channels + c;
 #pragma unroll
-            for (int j = 0; j < NPL; ++j) {
-                const float2 v = unpack2(h[j / 2]);
-                if (n0 + j < a.dstate) dst[static_cast<long long>(n0 + j) * a.channels] = j % 2 ? v.y : v.x;
-            }
+            for (int j = 0; j < NPL; ++j)
+                if (n0 + j < a.dstate) dst[static_cast<long long>(n0 + j) * a.channels] = h[j];
         }
-        // kGroup tokens at a time, the next ones' operands on their way: nothing but the states depends on the token before.
-        // Rows behind the last token have dt = 0; groups of nothing else are left out.
-        constexpr int kGroup = NPL <= 4 ? 4 : NPL <= 8 ? 2 : 1, kGroups = kScanTile / kGroup;
+        // kGroup tokens at a time.  Only the states depend on the token before: the operands of the next groups are on their
+        // way, and the next one's exponentials lie between the steps of this one's recurrence, all in one straight line.
+        // Groups of four or eight tokens take 4 to 10% longer: their loads and exponentials come in bursts.  Rows behind the
+        // last token have dt = 0; where they are half of the tile they are left out.
+                constexpr int kGroup = 2, kAhead = NPL <= 2 ? 2 : 1;
         struct Operands {
-            float2 du[kGroup];
-            ulonglong2 b[kGroup][NPL / 4], c[kGroup][NPL / 4];
+            float dt[kGroup], u[kGroup], b[NPL][kGroup], c[NPL][kGroup];
         };
-        const auto row_of = [](int i) { return kReverse ? kScanTile - 1 - i : i; };
-        const auto fetch = [&](Operands& o, int group) {
+        const auto walk = [&](auto rows) {
+            constexpr int kRows = decltype(rows)::value, kGroups = kRows / kGroup;
+            const auto fetch = [&](Operands& o, int group) {
+                const int first = (kReverse ? kGroups - 1 - group : group) * kGroup;
 #pragma unroll
-            for (int i = 0; i < kGroup; ++i) {
-                const int row = row_of(group * kGroup + i);
-                o.du[i] = sdu[row * channels_here + mine];
-#pragma unroll
-                for (int j = 0; j < NPL / 4; ++j) {
-                    o.b[i][j] = *reinterpret_cast<const ulonglong2*>(sb + row * kCols + n0 + 4 * j);
-                    if (kMode == kForward) o.c[i][j] = *reinterpret_cast<const ulonglong2*>(sc + row * kCols + n0 + 4 * j);
+                for (int i = 0; i < kGroup; i += 2) {
+                    const float4 du = sm.du[(first + i) / 2][lane];
+                    o.dt[i] = du.x, o.dt[i + 1] = du.y, o.u[i] = du.z, o.u[i + 1] = du.w;
                 }
-            }
-        };
-        Operands now, next;
-        fetch(now, 0);
 #pragma unroll
-        for (int group = 0; group < kGroups; ++group) {
-            if (!kReverse && group * kGroup >= nt) break;
-            if (group + 1 < kGroups) fetch(next, group + 1);
-            if (!kReverse || row_of(group * kGroup + kGroup - 1) < nt) {
-                F2 e[kGroup][NPL / 2];
-                float y[kGroup];
+                for (int j = 0; j < NPL; ++j) {
+                    const float2 bv = *reinterpret_cast<const float2*>(&sm.b[n0 + j][first]);
+                    o.b[j][0] = bv.x, o.b[j][1] = bv.y;
+                    if (kMode == kForward) {
+                        const float2 cv = *reinterpret_cast<const float2*>(&sm.c[kMode == kForward ? n0 + j : 0][first]);
+                        o.c[j][0] = cv.x, o.c[j][1] = cv.y;
+                    }
+                }
+            };
+            Operands now, next, third;
+            float e[NPL][kGroup], e_next[NPL][kGroup];
+            fetch(now, 0);
+            if (kAhead == 2 && kGroups > 1) fetch(next, 1);
 #pragma unroll
-                for (int i = 0; i < kGroup; ++i)
+            for (int j = 0; j < NPL; ++j)
 #pragma unroll
-                    for (int j = 0; j < NPL / 2; ++j) e[i][j] = exp2_2(mul2(pack2(now.du[i].x, now.du[i].x), a2[j]));
+                for (int i = 0; i < kGroup; ++i) e[j][i] = ex2f(now.dt[i] * a2[j]);
+#pragma unroll
+            for (int group = 0; group < kGroups; ++group) {
+                if (group + kAhead < kGroups) fetch(kAhead == 2 ? third : next, group + kAhead);
+                float in[NPL][kGroup], y[kGroup];
+#pragma unroll
+                for (int j = 0; j < NPL; ++j)
+#pragma unroll
+                    for (int i = 0; i < kGroup; ++i) {
+                        in[j][i] = now.u[i] * now.b[j][i];
+                        if (kReverse) in[j][i] *= e[j][i];
+                    }
 #pragma unroll
                 for (int i = 0; i < kGroup; ++i) {
-                    const F2 uu = pack2(now.du[i].y, now.du[i].y);
-                    if (kMode != kForward) sum_dt += now.du[i].x;
-                    F2 sum = 0;
+                    const int t = kReverse ? kGroup - 1 - i : i;
+                    if (kMode != kForward) sum_dt += now.dt[t];
 #pragma unroll
-                    for (int j = 0; j < NPL / 4; ++j) {
-                        const ulonglong2 bv = now.b[i][j];
-                        if (kReverse) {
-                            h[2 * j] = mul2(e[i][2 * j], fma2(uu, bv.x, h[2 * j]));
-                            h[2 * j + 1] = mul2(e[i][2 * j + 1], fma2(uu, bv.y, h[2 * j + 1]));
-                        } else {
-                            h[2 * j] = fma2(e[i][2 * j], h[2 * j], mul2(uu, bv.x));
-                            h[2 * j + 1] = fma2(e[i][2 * j + 1], h[2 * j + 1], mul2(uu, bv.y));
-                        }
-                        if (kMode == kForward) {
-                            sum = fma2(now.c[i][j].x, h[2 * j], sum);
-                            sum = fma2(now.c[i][j].y, h[2 * j + 1], sum);
-                        }
+                    for (int j = 0; j < NPL; ++j) {
+                        h[j] = fmaf(e[j][t], h[j], in[j][t]);
+                        if (kMode == kForward) y[t] = j == 0 ? now.c[0][t] * h[0] : fmaf(now.c[j][t], h[j], y[t]);
                     }
-                    y[i] = sum2(sum);
+                    if (group + 1 < kGroups) {
+#pragma unroll
+                        for (int j = 0; j < NPL; ++j) e_next[j][t] = ex2f(next.dt[t] * a2[j]);
+                    }
                 }
                 if (kMode == kForward) {
 #pragma unroll
-                    for (int i = 0; i < kGroup; ++i)
-                        sy[(wn * kScanTile + row_of(group * kGroup + i)) * channels_here + mine] = y[i];
+                    for (int i = 0; i < kGroup; i += 2)
+                        sm.y[kMode == kForward ? warp : 0][(group * kGroup + i) / 2][lane] = make_float2(y[i], y[i + 1]);
                 }
+#pragma unroll
+                for (int j = 0; j < NPL; ++j)
+#pragma unroll
+                    for (int i = 0; i < kGroup; ++i) e[j][i] = e_next[j][i];
+                now = next;
+                if (kAhead == 2) next = third;
             }
-            now = next;
-        }
+        };
+        if (nt > kScanTile / 2)
+            walk(std::integral_constant<int, kScanTile>{});
+        else
+            walk(std::integral_constant<int, kScanTile / 2>{});
         __syncthreads();
         if (kMode == kForward) {
+            T* to = out + static_cast<long long>(t0) * a.channels;
 #pragma unroll
-            for (int p = 0; p < kPairs; ++p) {
-                const int row = first_row + p * row_step;
-                if (row >= nt) continue;
-                float2 y = make_float2(skip.x * held[p].x, skip.y * held[p].y);
+            for (int p = 0; p < kPairs; p += 2) {
+                const int row = row_at(p);
+                float4 y = make_float4(skip.x * held[p].x, skip.x * held[p + 1].x, skip.y * held[p].y, skip.y * held[p + 1].y);
 #pragma unroll
                 for (int w = 0; w < NW; ++w) {
-                    const float2 v = *reinterpret_cast<const float2*>(&sy[(w * kScanTile + row) * channels_here + 2 * pair]);
-                    y.x += v.x;
-                    y.y += v.y;
+                    const float4 v = *reinterpret_cast<const float4*>(&sm.y[kMode == kForward ? w : 0][row / 2][2 * pair]);
+                    y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
                 }
-                if (a.z != nullptr) {
-                    const float2 zv = pair_f(zr[p]);
-                    y.x *= zv.x * sigmoid_fast(zv.x);
-                    y.y *= zv.y * sigmoid_fast(zv.y);
+                float2 o[2] = {make_float2(y.x, y.z), make_float2(y.y, y.w)};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (a.z != nullptr) {
+                        const float2 zv = pair_f(zr[p + i]);
+                        o[i].x *= zv.x * sigmoid_fast(zv.x);
+                        o[i].y *= zv.y * sigmoid_fast(zv.y);
+                    }
+                    store_pair<VECTOR>(to + static_cast<long long>(row + i) * a.channels, o[i], row + i < nt ? pn : 0);
                 }
-                store_pair<VECTOR>(out + static_cast<long long>(t0 + row) * a.channels + 2 * pair, y, pn);
             }
         }
     }
@@ -279,18 +286,14 @@ selective_walk_kernel(const SsdScanArgs a, const ScanLaunch l) {
         if (!s.last || a.final_state == nullptr) return;
         float* dst = a.final_state + (static_cast<long long>(s.seq) * a.channels + c) * a.dstate;
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) {
-            const float2 v = unpack2(h[j / 2]);
-            if (n0 + j < a.dstate) dst[n0 + j] = j % 2 ? v.y : v.x;
-        }
+        for (int j = 0; j < NPL; ++j)
+            if (n0 + j < a.dstate) dst[n0 + j] = h[j];
     } else {
         float* dst = l.work + item * a.dstate * a.channels + c;
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) {
-            const float2 v = unpack2(h[j / 2]);
-            if (n0 + j < a.dstate) dst[static_cast<long long>(n0 + j) * a.channels] = j % 2 ? v.y : v.x;
-        }
-        if (wn == 0) l.work[l.map.items() * a.dstate * a.channels + item * a.channels + c] = sum_dt;
+        for (int j = 0; j < NPL; ++j)
+            if (n0 + j < a.dstate) dst[static_cast<long long>(n0 + j) * a.channels] = h[j];
+        if (warp == 0) l.work[l.map.items() * a.dstate * a.channels + item * a.channels + c] = sum_dt;
     }
 }
 
@@ -325,40 +328,38 @@ selective_join_kernel(const SsdScanArgs a, const SeqMap map, float* work, const 
     }
 }
 
-// (columns of a warp, warps) for a number of state columns
+// (columns of a warp, warps) for a number of state columns.  `few`: no more CTAs than SMs, so that four columns per warp leave
+// a scheduler with one warp; two columns per warp then, although each warp reads dt and dt x again: 368 against 420 us
+// for [1,8192,4096] with 16 columns, but 152 against 147 us for [4,2000,2048], which has two CTAs on most SMs.
 template <class F>
-int with_columns(int dstate, F f) {
+int with_columns(int dstate, bool few, F f) {
     auto is = [&](auto npl, auto nw) { return f(npl, nw); };
+    if (dstate <= 8 && few) return is(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
     if (dstate <= 8) return is(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
+    if (dstate <= 16 && few) return is(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{});
     if (dstate <= 16) return is(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
-    if (dstate <= 32) return is(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
+    if (dstate <= 32) return is(std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
     if (dstate <= 64) return is(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
     return is(std::integral_constant<int, 16>{}, std::integral_constant<int, 8>{});
 }
 
 template <ScanMode kMode>
 int launch_walk(const SsdScanArgs& a, ScanLaunch l, bool pairs, cudaStream_t stream) {
+    l.blocks = scan_blocks(a.channels, a.groups, kWalkChannels);
+    const long long ctas = l.map.items() * l.blocks.count(a.groups);
+    if (ctas > 0x7fffffffLL) return SSD_ERR_RANGE;
     return with_type(a.dtype, [&](auto t) {
         using T = decltype(t);
-        return with_columns(a.dstate, [&](auto npl, auto nw) {
+        return with_columns(a.dstate, ctas <= sm_count(), [&](auto npl, auto nw) {
             constexpr int NPL = decltype(npl)::value, NW = decltype(nw)::value;
-            // sets of 32 channels in a CTA: several, up to 256 threads, only where that leaves two CTAs per SM
-            l.cg = NW >= 8 ? 1 : 8 / NW;
-            while (true) {
-                l.blocks = scan_blocks(a.channels, a.groups, 32 * l.cg);
-                if (l.cg == 1 || l.map.items() * l.blocks.count(a.groups) >= 2LL * sm_count()) break;
-                l.cg /= 2;
-            }
-            const long long ctas = l.map.items() * l.blocks.count(a.groups);
-            if (ctas > 0x7fffffffLL) return static_cast<int>(SSD_ERR_RANGE);
-            const size_t smem = sizeof(float) * kScanTile * (32 * l.cg * (2 + (kMode == kForward ? NW : 0)) + 2 * NPL * NW);
-            auto kernel = pairs ? selective_walk_kernel<T, NPL, NW, true, kMode> : selective_walk_kernel<T, NPL, NW, false, kMode>;
+            constexpr size_t smem = sizeof(WalkSmem<NPL, NW, kMode>);
+            const auto kernel = pairs ? selective_walk_kernel<T, NPL, NW, true, kMode> : selective_walk_kernel<T, NPL, NW, false, kMode>;
             if (smem > 48 * 1024) {
                 static std::atomic<uint64_t> done[2];
-                const int rc = set_max_smem_once(reinterpret_cast<const void*>(kernel), 96 * 1024, done[pairs]);
+                const int rc = set_max_smem_once(reinterpret_cast<const void*>(kernel), smem, done[pairs]);
                 if (rc != SSD_OK) return rc;
             }
-            launch_plain(kernel, static_cast<unsigned>(ctas), 32 * NW * l.cg, smem, stream, a, l);
+            launch_plain(kernel, static_cast<unsigned>(ctas), 32 * NW, smem, stream, a, l);
             return launch_status();
         });
     });
@@ -372,6 +373,8 @@ int scan_check(const SsdScanArgs& a) {
         return SSD_ERR_SHAPE;
     if (a.dstate > kScanMaxState || a.dtype < SSD_F32 || a.dtype > SSD_F16) return SSD_ERR_UNSUPPORTED;
     if (a.tokens > 0x7fffffff - (1 << 20) || a.rows > 0x7ffffff0) return SSD_ERR_RANGE;
+    for (const int64_t step : {a.x_strides[1], a.dt_strides[1], a.z_strides[1], a.b_strides[1], a.c_strides[1], int64_t{a.channels}})
+        if (step < 0 || step >= (1 << 29)) return SSD_ERR_RANGE;
     if (!a.A || (a.tokens > 0 && (!a.x || !a.dt || !a.bm || !a.cm))) return SSD_ERR_NULL;
     return SSD_OK;
 }
@@ -396,7 +399,7 @@ ScanSegments scan_segments(const SsdScanArgs& a, int per_cta, int slots) {
 
 int scan_segment_states(const SsdScanArgs& a, const ScanSegments& s, float* work, const void* dout, const float* dfinal,
                         cudaStream_t stream) {
-    ScanLaunch l{scan_map(a, s.span), {}, 1, true, work, dout};
+    ScanLaunch l{scan_map(a, s.span), {}, true, work, dout};
     const bool pairs = [&] {
         const size_t element = a.dtype == SSD_F32 ? 4 : 2;
         return scan_pairs(a, element) && aligned_to(2 * element, dout);
@@ -438,6 +441,6 @@ extern "C" int ssd_selective_scan_fwd(const SsdScanArgs* args, ssd_stream_t stre
         if (!a.work) return SSD_ERR_NULL;
         if (const int rc = scan_segment_states(a, s, a.work, nullptr, nullptr, st); rc != SSD_OK) return rc;
     }
-    const ScanLaunch l{scan_map(a, s.span), {}, 1, s.split, a.work, nullptr};
+    const ScanLaunch l{scan_map(a, s.span), {}, s.split, a.work, nullptr};
     return launch_walk<kForward>(a, l, scan_pairs(a, a.dtype == SSD_F32 ? 4 : 2), st);
 }

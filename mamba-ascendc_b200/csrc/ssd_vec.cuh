@@ -106,8 +106,13 @@ __device__ __forceinline__ float ex2f(float v) {
     return r;
 }
 constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float rcpf(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
 // 1 / (1 + e^-v): exact limits at both ends (e^-v overflows to infinity, whose reciprocal is 0)
-__device__ __forceinline__ float sigmoid_fast(float v) { return __fdividef(1.f, 1.f + ex2f(-v * kLog2e)); }
+__device__ __forceinline__ float sigmoid_fast(float v) { return rcpf(1.f + ex2f(-v * kLog2e)); }
 
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
