@@ -186,3 +186,21 @@ def check(code: int, op: str) -> None:
     """Raise the reference's style of error (``RuntimeError("<op>: <message>")``) for a failed call."""
     if code != SSD_OK:
         raise RuntimeError(f"{op}: {error_string(code)} (code {code})")
+
+
+def _load_calls():
+    """The extension module of csrc/torch_calls.cpp, bound to the library above."""
+    import importlib
+
+    import torch  # noqa: F401  (the module links against its libraries)
+
+    try:
+        module = importlib.import_module(__package__ + "._calls")
+    except ImportError as error:
+        raise ImportError(f"{Path(__file__).resolve().parent / '_calls.so'} is missing or belongs to another torch: build it with "
+                          f"`python mamba-ascendc_b200/build.py` ({error})") from error
+    module.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in SIGNATURES if hasattr(lib, name)})
+    return module
+
+
+calls = _load_calls()

@@ -1,4 +1,5 @@
-"""Checks of arguments that the operators around a selective state space layer share.
+"""Checks of arguments that the operators around a selective state space layer share: what a call says that ``_calls``
+(csrc/torch_calls.cpp, which checks the same) did not take.
 
 They raise ``RuntimeError("<operator>: ...")`` before any launch, as ``mamba2_ssd_fwd`` does
 (mamba_ascendc/csrc/ops/mamba2_ssd_fwd/op_host/mamba2_ssd_fwd.cpp:15-112)."""
@@ -8,13 +9,16 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import _capi
-
-DTYPES = {torch.float32: _capi.SSD_F32, torch.bfloat16: _capi.SSD_BF16, torch.float16: _capi.SSD_F16}
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def fail(op: str, text: str) -> None:
     raise RuntimeError(f"{op}: {text}")
+
+
+def unsupported(op: str) -> None:
+    """The arguments are as they should be, but a tensor is not a plain one (its storage, layout or device)."""
+    fail(op, "takes plain strided CUDA tensors only")
 
 
 def activation(op: str, t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:

@@ -1,4 +1,5 @@
-"""Build libssd_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a.
+"""Build libssd_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a, and beside it _calls.so (calls on torch tensors
+in front of it) with g++ against the headers of the installed torch.
 
 Usage: ``python mamba-ascendc_b200/build.py [--force] [--verbose]``.  The shared
 object is written next to the Python package so that ``ascend_kernel`` finds it
@@ -18,6 +19,8 @@ ROOT = Path(__file__).resolve().parent
 CSRC = ROOT / "csrc"
 OBJ_DIR = ROOT / "build"
 LIB_PATH = ROOT / "ascend_kernel" / "libssd_b200.so"
+CALLS_SOURCE = CSRC / "torch_calls.cpp"
+CALLS_PATH = ROOT / "ascend_kernel" / "_calls.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -47,6 +50,35 @@ def _sources(product_only: bool = False) -> list[Path]:
 def _deps_mtime() -> float:
     deps = list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + [ROOT.parent / "include" / "ssd_b200.h"]
     return max(p.stat().st_mtime for p in deps)
+
+
+def build_calls(force: bool = False) -> Path:
+    """The extension module of torch_calls.cpp: host code only."""
+    import sysconfig
+
+    import torch
+
+    header = ROOT.parent / "include" / "ssd_b200.h"
+    stamp = OBJ_DIR / ".calls"
+    want = f"{torch.__version__} {sysconfig.get_config_var('SOABI')}"
+    newest = max(CALLS_SOURCE.stat().st_mtime, header.stat().st_mtime)
+    if (not force and CALLS_PATH.exists() and CALLS_PATH.stat().st_mtime >= newest and stamp.exists() and
+            stamp.read_text() == want):
+        return CALLS_PATH
+    home = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parent.parent
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-DTORCH_EXTENSION_NAME=_calls",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{p}" for p in (home / "include", home / "include/torch/csrc/api/include", sysconfig.get_paths()["include"],
+                                cuda / "include")),
+           str(CALLS_SOURCE), "-o", str(CALLS_PATH), f"-L{home / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+           "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(" ".join(cmd) + "\n" + res.stdout + res.stderr)
+        raise RuntimeError(f"g++ failed for {CALLS_SOURCE}")
+    stamp.write_text(want)
+    return CALLS_PATH
 
 
 def build(force: bool = False, verbose: bool = False, product_only: bool = False) -> Path:
@@ -89,6 +121,7 @@ def build(force: bool = False, verbose: bool = False, product_only: bool = False
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("linking libssd_b200.so failed")
         flavour.write_text(want_flavour)
+    build_calls(force)
     return LIB_PATH
 
 
