@@ -110,7 +110,7 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
         if (kOut == kOneScale) scale = *static_cast<const float*>(a.static_scale);
         if (kOut == kRowScale) {
             // rstd is positive, so the largest |v w| is the largest |out| but for rstd
-            scale = red.top * rstd / 448.f;
+            scale = red.top * rstd * (1.f / 448.f);
             if (scale == 0.f) scale = 1.f;
             if (live && at == 0) a.scales[row] = scale;
         }
@@ -126,16 +126,16 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) m = max_nan(m, fabsf(y[j]));
                 for (int o = a.group / VEC / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                scale = m / 448.f;
+                scale = m * (1.f / 448.f);
                 if (scale == 0.f) scale = 1.f;
                 if (n > 0 && c % a.group == 0) a.scales[row * (a.width / a.group) + c / a.group] = scale;
             }
-            // a reciprocal, but for scales so small that it would overflow
+            // times the reciprocal (one step off at most), but for scales so small that it would overflow
             if (fabsf(scale) < 1e-30f) {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) y[j] = y[j] / scale;
             } else {
-                const float inv = 1.f / scale;
+                const float inv = rcpf(scale);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) y[j] *= inv;
             }

@@ -1,66 +1,105 @@
 // Selective scan of one token of each sequence: the state out of a cache, moved on by the token, and back.
 //
-// What bounds it: HBM, the state once in each direction (fp32, 4 dstate bytes per channel each way against 8 of the token).
-// Lanes lie along the state (four columns each) and then along the channels, so that a warp reads and writes whole lines;
-// a thread takes kRows rows of the batch with the loads of all their states in flight, and keeps A.
+// What bounds it: HBM, the state once in each direction (fp32, 4 dstate bytes per channel each way against 8 of the token),
+// as long as little else is done per state column: what belongs to a (row, channel), softplus, gate and skip connection, is
+// formed once by one thread and passes to the channel's lanes through shared memory, as do B and C in fp32.  A lane has eight
+// columns of a channel (32 bytes, one access), lanes lie along the columns and then along the channels; a thread takes
+// ROWS rows of the batch with the loads of all their states in flight, and keeps A.
 #include "ssd_selective.cuh"
 
 namespace ssd {
 
 namespace {
 
-constexpr int kStepThreads = 128;
+constexpr int kStepThreads = 128, kStepCols = 8;
 
-// LPC lanes hold a channel's columns, four each.  VECTOR: dstate is a multiple of four, and states, B and C
-// are aligned for four at once.
+// Eight floats at a 32-byte boundary.
+__device__ __forceinline__ void load8(float (&f)[kStepCols], const float* p) {
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void store8(float* p, const float (&f)[kStepCols]) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]),
+                 "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+                 : "memory");
+}
+
+// LPC lanes hold a channel's columns.  VECTOR: dstate is a multiple of eight and the states lie at 32-byte boundaries.
 template <class T, int LPC, int ROWS, bool VECTOR>
 __global__ void __launch_bounds__(kStepThreads)
-selective_step_kernel(const SsdScanStepArgs a, int channel_blocks) {
-    constexpr int kChannels = kStepThreads / LPC;
+selective_step_kernel(const SsdScanStepArgs a, const ScanBlocks b) {
+    constexpr int kChannels = kStepThreads / LPC, kWide = LPC * kStepCols;  // channels of a CTA, columns with those behind dstate
     __shared__ unsigned flags;  // bit i: row i's slot is taken by an earlier row; bit 16 + i: a later row names it too
-    const int row0 = blockIdx.x / channel_blocks * ROWS;
-    const int c = blockIdx.x % channel_blocks * kChannels + threadIdx.x / LPC;
-    const int part = threadIdx.x % LPC, n0 = part * 4, nn = max(min(a.dstate - n0, 4), 0);
-    const bool live = c < a.channels;
-    const int g = live ? c / (a.channels / a.groups) : 0;
+    __shared__ float4 token[ROWS][kChannels];  // dt, dt x, gate, gated skip connection
+    __shared__ __align__(16) float shared[ROWS][2][kWide];
+    const int blocks = b.count(a.groups), row0 = blockIdx.x / blocks * ROWS, tid = threadIdx.x;
+    const ChannelBlock cb = channel_block(b, blockIdx.x % blocks, a.channels, a.groups);
+    const int mine = tid / LPC, c = cb.first + mine, part = tid % LPC, n0 = part * kStepCols;
+    const int nn = mine < cb.n ? max(min(a.dstate - n0, kStepCols), 0) : 0;
+    const long long own = static_cast<long long>(c) * a.dstate + n0;
 
-    // every load of the rows in flight before the first is used
     long long slot[ROWS];
-    Pack<float, 4> hr[ROWS];
-    Pack<T, 4> br[ROWS], cr[ROWS];
-    Pack<T, 1> xr[ROWS], dr[ROWS], zr[ROWS];
-    auto request = [&](Pack<T, 1>& xv, Pack<T, 1>& dv, Pack<T, 1>& zv, Pack<T, 4>& bv, Pack<T, 4>& cv, long long row, bool in) {
-        load_raw<true, false>(xv, static_cast<const T*>(a.x) + row * a.x_stride + c, in);
-        load_raw<true, false>(dv, static_cast<const T*>(a.dt) + row * a.dt_stride + c, in);
-        load_raw<true, false>(zv, static_cast<const T*>(a.z) + row * a.z_stride + c, in && a.z != nullptr);
-        load_raw<VECTOR, false>(bv, static_cast<const T*>(a.bm) + row * a.b_strides[0] + g * a.b_strides[1] + n0, in ? nn : 0);
-        load_raw<VECTOR, false>(cv, static_cast<const T*>(a.cm) + row * a.c_strides[0] + g * a.c_strides[1] + n0, in ? nn : 0);
-    };
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int row = row0 + i;
         slot[i] = row >= a.rows ? -1 : a.slots != nullptr ? a.slots[row] : row;
         if (slot[i] >= a.slot_count) slot[i] = -1;
     }
+    float h[ROWS][kStepCols], a2[kStepCols];
+    const auto load_state = [&](float (&f)[kStepCols], const float* p, bool in) {
+        if constexpr (VECTOR) {
+            if (in && nn > 0) {
+                load8(f, p);
+            } else {
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        const bool in = live && slot[i] >= 0;
-        load_raw<VECTOR, true>(hr[i], a.state + (in ? slot[i] * a.state_stride + static_cast<long long>(c) * a.dstate + n0 : 0),
-                               in ? nn : 0);
-        request(xr[i], dr[i], zr[i], br[i], cr[i], in ? row0 + i : 0, in);
-    }
-    float a2[4];
-    load_f<VECTOR>(a2, a.A + (live ? static_cast<long long>(c) * a.dstate + n0 : 0), live ? nn : 0);
+                for (int j = 0; j < kStepCols; ++j) f[j] = 0.f;
+            }
+        } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a2[j] *= kLog2e;
-    const float bias = live && a.dt_bias != nullptr ? a.dt_bias[c] : 0.f, skip = live && a.D != nullptr ? a.D[c] : 0.f;
+            for (int j = 0; j < kStepCols; ++j) f[j] = in && j < nn ? p[j] : 0.f;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) load_state(h[i], a.state + slot[i] * a.state_stride + own, slot[i] >= 0);
 
+    // what belongs to a token: one thread per (row, channel), and per (row, column) of B and C
+    const auto stage = [&](int i, int row) {
+        for (int k = tid; k < kChannels; k += kStepThreads) {
+            if (k >= cb.n) break;
+            const int ch = cb.first + k;
+            const float xv = to_f(static_cast<const T*>(a.x)[row * a.x_stride + ch]);
+            float d = to_f(static_cast<const T*>(a.dt)[row * a.dt_stride + ch]);
+            float gate = 1.f;
+            if (a.z != nullptr) {
+                const float zv = to_f(static_cast<const T*>(a.z)[row * a.z_stride + ch]);
+                gate = zv * sigmoid_fast(zv);
+            }
+            if (a.dt_bias != nullptr) d += a.dt_bias[ch];
+            if (a.softplus) d = softplus_series(d);
+            const float skip = a.D != nullptr ? a.D[ch] * xv : 0.f;
+            token[i][k] = make_float4(d, d * xv, gate, skip);
+        }
+        for (int k = tid; k < 2 * kWide; k += kStepThreads) {
+            const int n = k % kWide;
+            const bool second = k >= kWide;
+            const T* src = static_cast<const T*>(second ? a.cm : a.bm) + row * (second ? a.c_strides[0] : a.b_strides[0]) +
+                           cb.group * (second ? a.c_strides[1] : a.b_strides[1]);
+            shared[i][second][n] = n < a.dstate ? to_f(src[n]) : 0.f;
+        }
+    };
+    if (tid == 0) flags = 0;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+        if (slot[i] >= 0) stage(i, row0 + i);
+    load_state(a2, a.A + own, true);
+#pragma unroll
+    for (int j = 0; j < kStepCols; ++j) a2[j] *= kLog2e;
+    __syncthreads();
     unsigned found = 0;
     if (a.slots != nullptr) {
-        if (threadIdx.x == 0) flags = 0;
-        __syncthreads();
         unsigned bits = 0;
-        for (int r = threadIdx.x; r < a.rows; r += kStepThreads) {
+        for (int r = tid; r < a.rows; r += kStepThreads) {
             const int other = a.slots[r];
 #pragma unroll
             for (int i = 0; i < ROWS; ++i)
@@ -72,53 +111,51 @@ selective_step_kernel(const SsdScanStepArgs a, int channel_blocks) {
     }
 
     // one token: the state moved on, and its output
-    auto token = [&](float (&s)[4], const Pack<T, 1>& xp, const Pack<T, 1>& dp, const Pack<T, 1>& zp, const Pack<T, 4>& bp,
-                     const Pack<T, 4>& cp, int row) {
-        float b[4], cv[4];
-        unpack(b, bp);
-        unpack(cv, cp);
-        const float xv = to_f(xp.v[0]);
-        float d = to_f(dp.v[0]) + bias;
-        if (a.softplus) d = softplus_series(d);
-        const float u = d * xv;
+    const auto step = [&](float (&s)[kStepCols], int i, int row) {
+        const float4 t = token[i][mine];
         float y = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            s[j] = fmaf(ex2f(d * a2[j]), s[j], u * b[j]);
-            y = fmaf(cv[j], s[j], y);
+        for (int j = 0; j < kStepCols; j += 4) {
+            const float4 bv = *reinterpret_cast<const float4*>(&shared[i][0][n0 + j]);
+            const float4 cv = *reinterpret_cast<const float4*>(&shared[i][1][n0 + j]);
+            const float bs[4] = {bv.x, bv.y, bv.z, bv.w}, cs[4] = {cv.x, cv.y, cv.z, cv.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                s[j + k] = fmaf(ex2f(t.x * a2[j + k]), s[j + k], t.y * bs[k]);
+                y = fmaf(cs[k], s[j + k], y);
+            }
         }
 #pragma unroll
         for (int o = LPC / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-        if (live && part == 0) {
-            y = fmaf(skip, xv, y);
-            if (a.z != nullptr) {
-                const float zv = to_f(zp.v[0]);
-                y *= zv * sigmoid_fast(zv);
-            }
-            static_cast<T*>(a.out)[static_cast<long long>(row) * a.channels + c] = from_f<T>(y);
-        }
+        if (part == 0 && mine < cb.n)
+            static_cast<T*>(a.out)[static_cast<long long>(row) * a.channels + c] = from_f<T>((y + t.w) * t.z);
     };
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int row = row0 + i;
         if (row >= a.rows) break;
         if (slot[i] < 0) {
-            if (live && part == 0) static_cast<T*>(a.out)[static_cast<long long>(row) * a.channels + c] = from_f<T>(0.f);
+            if (part == 0 && mine < cb.n) static_cast<T*>(a.out)[static_cast<long long>(row) * a.channels + c] = from_f<T>(0.f);
             continue;
         }
         if (found & (1u << i)) continue;  // the first row with this slot takes them all
-        float h[4];
-        unpack(h, hr[i]);
-        token(h, xr[i], dr[i], zr[i], br[i], cr[i], row);
+        step(h[i], i, row);
         if (found & (0x10000u << i))
             for (int r = row + 1; r < a.rows; ++r)
                 if (a.slots[r] == slot[i]) {
-                    Pack<T, 1> xv, dv, zv;
-                    Pack<T, 4> bv, cv;
-                    request(xv, dv, zv, bv, cv, r, live);
-                    token(h, xv, dv, zv, bv, cv, r);
+                    __syncthreads();  // the same for the whole CTA
+                    stage(i, r);
+                    __syncthreads();
+                    step(h[i], i, r);
                 }
-        if (live) store_f<VECTOR>(a.state_out + slot[i] * a.state_out_stride + static_cast<long long>(c) * a.dstate + n0, h, nn);
+        float* dst = a.state_out + slot[i] * a.state_out_stride + own;
+        if constexpr (VECTOR) {
+            if (nn > 0) store8(dst, h[i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kStepCols; ++j)
+                if (j < nn) dst[j] = h[i][j];
+        }
     }
 }
 
@@ -135,31 +172,30 @@ extern "C" int ssd_selective_scan_step(const SsdScanStepArgs* args, ssd_stream_t
         return SSD_ERR_SHAPE;
     if (a.dstate > kScanMaxState) return SSD_ERR_UNSUPPORTED;
     if (!a.x || !a.dt || !a.A || !a.bm || !a.cm || !a.state || !a.state_out || !a.out) return SSD_ERR_NULL;
-    const bool vector = a.dstate % 4 == 0 && aligned16(a.A, a.state, a.state_out) && multiple_of(a.state_stride, 4) &&
-                        multiple_of(a.state_out_stride, 4) && multiple_of(a.b_strides[0] | a.b_strides[1], 4) &&
-                        multiple_of(a.c_strides[0] | a.c_strides[1], 4) &&
-                        aligned_to(a.dtype == SSD_F32 ? 16 : 8, a.bm, a.cm);
+    const bool vector = a.dstate % kStepCols == 0 && aligned_to(32, a.A, a.state, a.state_out) &&
+                        multiple_of(a.state_stride, kStepCols) && multiple_of(a.state_out_stride, kStepCols);
     return with_type(a.dtype, [&](auto t) {
         using T = decltype(t);
-        const auto launch = [&](auto lpc, auto rows) {
-            constexpr int LPC = decltype(lpc)::value, ROWS = decltype(rows)::value;
-            const int channel_blocks = (a.channels + kStepThreads / LPC - 1) / (kStepThreads / LPC);
-            const long long blocks = static_cast<long long>((a.rows + ROWS - 1) / ROWS) * channel_blocks;
-            if (blocks > 0x7fffffffLL) return static_cast<int>(SSD_ERR_RANGE);
-            launch_plain(vector ? selective_step_kernel<T, LPC, ROWS, true> : selective_step_kernel<T, LPC, ROWS, false>,
-                         static_cast<unsigned>(blocks), kStepThreads, 0, reinterpret_cast<cudaStream_t>(stream), a, channel_blocks);
+        const auto with_rows = [&](auto lpc) {
+            constexpr int LPC = decltype(lpc)::value;
+            const ScanBlocks b = scan_blocks(a.channels, a.groups, kStepThreads / LPC);
+            // several rows of a thread share A; one where that would leave SMs without a CTA
+            const int rows = static_cast<long long>(a.rows) * b.count(a.groups) >= 16LL * sm_count() ? 4 : 1;
+            const long long ctas = static_cast<long long>((a.rows + rows - 1) / rows) * b.count(a.groups);
+            if (ctas > 0x7fffffffLL) return static_cast<int>(SSD_ERR_RANGE);
+            const auto launch = [&](auto kernel) {
+                launch_plain(kernel, static_cast<unsigned>(ctas), kStepThreads, 0, reinterpret_cast<cudaStream_t>(stream), a, b);
+            };
+            if (rows > 1)
+                vector ? launch(selective_step_kernel<T, LPC, 4, true>) : launch(selective_step_kernel<T, LPC, 4, false>);
+            else
+                vector ? launch(selective_step_kernel<T, LPC, 1, true>) : launch(selective_step_kernel<T, LPC, 1, false>);
             return launch_status();
         };
-        const auto with_rows = [&](auto lpc) {
-            // several rows of a thread share A; one where that would leave SMs without a CTA
-            constexpr int LPC = decltype(lpc)::value;
-            const long long ctas = static_cast<long long>(a.rows) * ((a.channels + kStepThreads / LPC - 1) / (kStepThreads / LPC));
-            return ctas >= 16LL * sm_count() ? launch(lpc, std::integral_constant<int, 4>{})
-                                             : launch(lpc, std::integral_constant<int, 1>{});
-        };
-        if (a.dstate <= 16) return with_rows(std::integral_constant<int, 4>{});
-        if (a.dstate <= 32) return with_rows(std::integral_constant<int, 8>{});
-        if (a.dstate <= 64) return with_rows(std::integral_constant<int, 16>{});
-        return with_rows(std::integral_constant<int, 32>{});
+        if (a.dstate <= 8) return with_rows(std::integral_constant<int, 1>{});
+        if (a.dstate <= 16) return with_rows(std::integral_constant<int, 2>{});
+        if (a.dstate <= 32) return with_rows(std::integral_constant<int, 4>{});
+        if (a.dstate <= 64) return with_rows(std::integral_constant<int, 8>{});
+        return with_rows(std::integral_constant<int, 16>{});
     });
 }

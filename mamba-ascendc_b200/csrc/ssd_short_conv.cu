@@ -353,27 +353,22 @@ int with_width(int width, F f) {
         default: return f(std::integral_constant<int, 4>{});
     }
 }
-// Tokens of an item of the forward pass: as many as leave about six CTAs per SM, so that little is read twice.
-int conv_span(const SsdConvArgs& a, int channel_blocks) {
-    const long long total = a.cu_seqlens ? a.tokens : a.tokens * a.rows;
-    int span = 64;
-    while (span > 8 && total / span * channel_blocks < 6LL * sm_count()) span /= 2;
-    return span;
+// Tokens of an item, so that the items are the CTAs that the SMs hold at a time, `resident` each: the filters are staged and
+// the W-1 tokens in front read once for as many tokens as that allows.
+int conv_span(const SsdConvArgs& a, int channel_blocks, int resident, int least) {
+    const long long ctas = (static_cast<long long>(resident) * sm_count() + channel_blocks - 1) / channel_blocks;
+    const long long sequences = a.cu_seqlens ? 1 : a.rows, per = ctas > sequences ? ctas / sequences : 1;
+    const long long span = (a.tokens + per - 1) / per;
+    return static_cast<int>(span < least ? least : span);
 }
-// Backward, the CTAs that the SMs hold at a time (three each, by registers) are dealt one item each where the sequences allow.
-constexpr int kConvGradCtas = 3;
-long long conv_grad_slices(int channel_blocks) {
-    return (static_cast<long long>(kConvGradCtas) * sm_count() + channel_blocks - 1) / channel_blocks;
-}
+// Backward, those CTAs (three per SM, by registers) are dealt one item each where the sequences allow.
+constexpr int kConvCtas = 4, kConvGradCtas = 3;
 ConvDims conv_grad_dims(const SsdConvArgs& a) {
     const int blocks = (a.channels + kConvThreads * kConvVec - 1) / (kConvThreads * kConvVec);
-    const long long slices = conv_grad_slices(blocks), sequences = a.cu_seqlens ? 1 : a.rows;
-    const long long per = slices > sequences ? slices / sequences : 1;
-    const long long span = (a.tokens + per - 1) / per;
-    return ConvDims{{a.cu_seqlens, a.tokens, a.rows, static_cast<int>(span < 16 ? 16 : span)}, blocks};
+    return ConvDims{{a.cu_seqlens, a.tokens, a.rows, conv_span(a, blocks, kConvGradCtas, 16)}, blocks};
 }
 int conv_slices(const ConvDims& d) {
-    const long long items = d.map.items(), fill = conv_grad_slices(d.channel_blocks);
+    const long long items = d.map.items(), fill = (static_cast<long long>(kConvGradCtas) * sm_count() + d.channel_blocks - 1) / d.channel_blocks;
     return static_cast<int>(items < fill ? items : fill);
 }
 
@@ -391,7 +386,7 @@ extern "C" int ssd_short_conv_fwd(const SsdConvArgs* args, ssd_stream_t stream) 
         using T = decltype(t);
         constexpr int V = kConvVec;
         const int channel_blocks = (a.channels + kConvThreads * V - 1) / (kConvThreads * V);
-        const ConvDims d{{a.cu_seqlens, a.tokens, a.rows, conv_span(a, channel_blocks)}, channel_blocks};
+        const ConvDims d{{a.cu_seqlens, a.tokens, a.rows, conv_span(a, channel_blocks, kConvCtas, 8)}, channel_blocks};
         const long long blocks = d.map.items() * channel_blocks;
         if (blocks > 0x7fffffffLL) return static_cast<int>(SSD_ERR_RANGE);
         const bool vector = aligned_to(sizeof(T) * V, a.x, a.initial_state, a.out, a.final_state) && multiple_of(a.channels, V) &&

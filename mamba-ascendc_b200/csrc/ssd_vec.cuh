@@ -21,6 +21,13 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return
 template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
+__device__ __forceinline__ void pair_from_f(__nv_bfloat16* p, float a, float b) {
+    *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b);
+}
+__device__ __forceinline__ void pair_from_f(__half* p, float a, float b) {
+    *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b);
+}
+
 // The plain vector of BYTES bytes.
 template <int BYTES>
 struct Bits;
@@ -82,8 +89,13 @@ __device__ __forceinline__ void store_raw(T* p, const Pack<T, V>& raw, int n) {
 template <bool VECTOR, int V, class T>
 __device__ __forceinline__ void store_f(T* p, const float (&f)[V], int n) {
     Pack<T, V> raw;
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {  // two values a conversion
 #pragma unroll
-    for (int i = 0; i < V; ++i) raw.v[i] = from_f<T>(f[i]);
+        for (int i = 0; i < V; i += 2) pair_from_f(raw.v + i, f[i], f[i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) raw.v[i] = from_f<T>(f[i]);
+    }
     store_raw<VECTOR>(p, raw, n);
 }
 
