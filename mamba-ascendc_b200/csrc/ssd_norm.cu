@@ -128,7 +128,8 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
                 for (int o = a.group / VEC / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
                 scale = m * (1.f / 448.f);
                 if (scale == 0.f) scale = 1.f;
-                if (n > 0 && c % a.group == 0) a.scales[row * (a.width / a.group) + c / a.group] = scale;
+                const int lg = 31 - __clz(a.group);
+                if (n > 0 && (c & (a.group - 1)) == 0) a.scales[row * (a.width >> lg) + (c >> lg)] = scale;
             }
             // times the reciprocal (one step off at most), but for scales so small that it would overflow
             if (fabsf(scale) < 1e-30f) {
@@ -141,9 +142,10 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
             }
             alignas(8) unsigned char q[VEC];
 #pragma unroll
-            for (int j = 0; j < VEC; j += 2)
-                *reinterpret_cast<unsigned short*>(q + j) =
-                    __nv_cvt_float2_to_fp8x2(make_float2(y[j], y[j + 1]), __NV_SATFINITE, __NV_E4M3);
+            for (int j = 0; j < VEC; j += 4)
+                *reinterpret_cast<unsigned*>(q + j) =
+                    __nv_cvt_float2_to_fp8x2(make_float2(y[j], y[j + 1]), __NV_SATFINITE, __NV_E4M3) |
+                    static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y[j + 2], y[j + 3]), __NV_SATFINITE, __NV_E4M3)) << 16;
             unsigned char* dst = static_cast<unsigned char*>(a.q) + row * a.width + c;
             if constexpr (VECTOR) {
                 using B = typename Bits<VEC>::type;

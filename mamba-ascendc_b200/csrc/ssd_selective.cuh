@@ -53,7 +53,8 @@ struct ChannelBlock {
     int group, first, n;  // first channel and how many there are
 };
 __device__ __forceinline__ ChannelBlock channel_block(const ScanBlocks& b, int block, int channels, int groups) {
-    const int mine = channels / groups, group = block / b.per_group, at = (block - group * b.per_group) * b.per_cta;
+    const int mine = groups == 1 ? channels : channels / groups, group = groups == 1 ? 0 : block / b.per_group;
+    const int at = (block - group * b.per_group) * b.per_cta;
     return {group, group * mine + at, min(mine - at, b.per_cta)};
 }
 
@@ -74,17 +75,6 @@ __device__ __forceinline__ void store_pair(T* p, float2 v, int n) {
     store_f<VECTOR>(p, f, n);
 }
 
-// Rows at a distance that fits 31 bits in bytes (scan_check), so that a row's address is one multiply-add.
-template <class T>
-struct Rows {
-    const char* base;
-    int step;
-    __device__ __forceinline__ Rows(const T* first, int64_t elements)
-        : base(reinterpret_cast<const char*>(first)), step(static_cast<int>(elements) * static_cast<int>(sizeof(T))) {}
-    __device__ __forceinline__ const T* at(int t) const {
-        return reinterpret_cast<const T*>(base + static_cast<long long>(t) * step);
-    }
-};
 // Token 0 of the sequence: the distance in elements from the tensor's start.
 __device__ __forceinline__ long long first_row(const SeqMap& m, const Span& s, const int64_t* strides) {
     return m.cu == nullptr ? s.seq * strides[0] : s.origin * strides[1];

@@ -33,13 +33,13 @@ selective_step_kernel(const SsdScanStepArgs a, const ScanBlocks b) {
     __shared__ unsigned flags;  // bit i: row i's slot is taken by an earlier row; bit 16 + i: a later row names it too
     __shared__ float4 token[ROWS][kChannels];  // dt, dt x, gate, gated skip connection
     __shared__ __align__(16) float shared[ROWS][2][kWide];
-    const int blocks = b.count(a.groups), row0 = blockIdx.x / blocks * ROWS, tid = threadIdx.x;
-    const ChannelBlock cb = channel_block(b, blockIdx.x % blocks, a.channels, a.groups);
+    const int row0 = blockIdx.x * ROWS, tid = threadIdx.x;
+    const ChannelBlock cb = channel_block(b, blockIdx.y, a.channels, a.groups);
     const int mine = tid / LPC, c = cb.first + mine, part = tid % LPC, n0 = part * kStepCols;
     const int nn = mine < cb.n ? max(min(a.dstate - n0, kStepCols), 0) : 0;
     const long long own = static_cast<long long>(c) * a.dstate + n0;
 
-    long long slot[ROWS];
+    int slot[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int row = row0 + i;
@@ -61,18 +61,21 @@ selective_step_kernel(const SsdScanStepArgs a, const ScanBlocks b) {
         }
     };
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) load_state(h[i], a.state + slot[i] * a.state_stride + own, slot[i] >= 0);
+    for (int i = 0; i < ROWS; ++i) load_state(h[i], a.state + static_cast<long long>(slot[i]) * a.state_stride + own, slot[i] >= 0);
 
     // what belongs to a token: one thread per (row, channel), and per (row, column) of B and C
-    const auto stage = [&](int i, int row) {
-        for (int k = tid; k < kChannels; k += kStepThreads) {
-            if (k >= cb.n) break;
+    const Rows<T> xs(static_cast<const T*>(a.x) + cb.first, a.x_stride), dts(static_cast<const T*>(a.dt) + cb.first, a.dt_stride);
+    const Rows<T> zs(static_cast<const T*>(a.z) + cb.first, a.z_stride);
+    const Rows<T> bs(static_cast<const T*>(a.bm) + cb.group * a.b_strides[1], a.b_strides[0]);
+    const Rows<T> cs(static_cast<const T*>(a.cm) + cb.group * a.c_strides[1], a.c_strides[0]);
+    const auto stage_token = [&](int i, int row, int k) {
+        if (k < cb.n) {
             const int ch = cb.first + k;
-            const float xv = to_f(static_cast<const T*>(a.x)[row * a.x_stride + ch]);
-            float d = to_f(static_cast<const T*>(a.dt)[row * a.dt_stride + ch]);
+            const float xv = to_f(__ldg(xs.at(row) + k));
+            float d = to_f(__ldg(dts.at(row) + k));
             float gate = 1.f;
             if (a.z != nullptr) {
-                const float zv = to_f(static_cast<const T*>(a.z)[row * a.z_stride + ch]);
+                const float zv = to_f(__ldg(zs.at(row) + k));
                 gate = zv * sigmoid_fast(zv);
             }
             if (a.dt_bias != nullptr) d += a.dt_bias[ch];
@@ -80,18 +83,19 @@ selective_step_kernel(const SsdScanStepArgs a, const ScanBlocks b) {
             const float skip = a.D != nullptr ? a.D[ch] * xv : 0.f;
             token[i][k] = make_float4(d, d * xv, gate, skip);
         }
-        for (int k = tid; k < 2 * kWide; k += kStepThreads) {
-            const int n = k % kWide;
-            const bool second = k >= kWide;
-            const T* src = static_cast<const T*>(second ? a.cm : a.bm) + row * (second ? a.c_strides[0] : a.b_strides[0]) +
-                           cb.group * (second ? a.c_strides[1] : a.b_strides[1]);
-            shared[i][second][n] = n < a.dstate ? to_f(src[n]) : 0.f;
-        }
+    };
+    const auto stage_shared = [&](int i, int row, int k) {
+        const int n = k % kWide;
+        shared[i][k / kWide][n] = n < a.dstate ? to_f(__ldg((k < kWide ? bs : cs).at(row) + n)) : 0.f;
     };
     if (tid == 0) flags = 0;
+    // all threads, whatever the row: a row of padding is staged as its slot would be
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-        if (slot[i] >= 0) stage(i, row0 + i);
+    for (int k = tid; k < ROWS * kChannels; k += kStepThreads)
+        if (row0 + k / kChannels < a.rows) stage_token(k / kChannels, row0 + k / kChannels, k % kChannels);
+#pragma unroll
+    for (int k = tid; k < ROWS * 2 * kWide; k += kStepThreads)
+        if (row0 + k / (2 * kWide) < a.rows) stage_shared(k / (2 * kWide), row0 + k / (2 * kWide), k % (2 * kWide));
     load_state(a2, a.A + own, true);
 #pragma unroll
     for (int j = 0; j < kStepCols; ++j) a2[j] *= kLog2e;
@@ -118,11 +122,11 @@ selective_step_kernel(const SsdScanStepArgs a, const ScanBlocks b) {
         for (int j = 0; j < kStepCols; j += 4) {
             const float4 bv = *reinterpret_cast<const float4*>(&shared[i][0][n0 + j]);
             const float4 cv = *reinterpret_cast<const float4*>(&shared[i][1][n0 + j]);
-            const float bs[4] = {bv.x, bv.y, bv.z, bv.w}, cs[4] = {cv.x, cv.y, cv.z, cv.w};
+            const float b4[4] = {bv.x, bv.y, bv.z, bv.w}, c4[4] = {cv.x, cv.y, cv.z, cv.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                s[j + k] = fmaf(ex2f(t.x * a2[j + k]), s[j + k], t.y * bs[k]);
-                y = fmaf(cs[k], s[j + k], y);
+                s[j + k] = fmaf(ex2f(t.x * a2[j + k]), s[j + k], t.y * b4[k]);
+                y = fmaf(c4[k], s[j + k], y);
             }
         }
 #pragma unroll
@@ -144,11 +148,12 @@ selective_step_kernel(const SsdScanStepArgs a, const ScanBlocks b) {
             for (int r = row + 1; r < a.rows; ++r)
                 if (a.slots[r] == slot[i]) {
                     __syncthreads();  // the same for the whole CTA
-                    stage(i, r);
+                    for (int k = tid; k < kChannels; k += kStepThreads) stage_token(i, r, k);
+                    for (int k = tid; k < 2 * kWide; k += kStepThreads) stage_shared(i, r, k);
                     __syncthreads();
                     step(h[i], i, r);
                 }
-        float* dst = a.state_out + slot[i] * a.state_out_stride + own;
+        float* dst = a.state_out + static_cast<long long>(slot[i]) * a.state_out_stride + own;
         if constexpr (VECTOR) {
             if (nn > 0) store8(dst, h[i]);
         } else {
@@ -171,6 +176,8 @@ extern "C" int ssd_selective_scan_step(const SsdScanStepArgs* args, ssd_stream_t
         (a.slots == nullptr && a.slot_count < a.rows))
         return SSD_ERR_SHAPE;
     if (a.dstate > kScanMaxState) return SSD_ERR_UNSUPPORTED;
+    if (!row_steps(a.x_stride, a.dt_stride, a.z_stride, a.b_strides[0], a.c_strides[0]) || a.state_stride < 0 || a.state_out_stride < 0)
+        return SSD_ERR_RANGE;
     if (!a.x || !a.dt || !a.A || !a.bm || !a.cm || !a.state || !a.state_out || !a.out) return SSD_ERR_NULL;
     const bool vector = a.dstate % kStepCols == 0 && aligned_to(32, a.A, a.state, a.state_out) &&
                         multiple_of(a.state_stride, kStepCols) && multiple_of(a.state_out_stride, kStepCols);
@@ -181,10 +188,10 @@ extern "C" int ssd_selective_scan_step(const SsdScanStepArgs* args, ssd_stream_t
             const ScanBlocks b = scan_blocks(a.channels, a.groups, kStepThreads / LPC);
             // several rows of a thread share A; one where that would leave SMs without a CTA
             const int rows = static_cast<long long>(a.rows) * b.count(a.groups) >= 16LL * sm_count() ? 4 : 1;
-            const long long ctas = static_cast<long long>((a.rows + rows - 1) / rows) * b.count(a.groups);
-            if (ctas > 0x7fffffffLL) return static_cast<int>(SSD_ERR_RANGE);
+            const dim3 grid((a.rows + rows - 1) / rows, b.count(a.groups));
+            if (grid.y > 65535u) return static_cast<int>(SSD_ERR_RANGE);
             const auto launch = [&](auto kernel) {
-                launch_plain(kernel, static_cast<unsigned>(ctas), kStepThreads, 0, reinterpret_cast<cudaStream_t>(stream), a, b);
+                launch_plain(kernel, grid, kStepThreads, 0, reinterpret_cast<cudaStream_t>(stream), a, b);
             };
             if (rows > 1)
                 vector ? launch(selective_step_kernel<T, LPC, 4, true>) : launch(selective_step_kernel<T, LPC, 4, false>);

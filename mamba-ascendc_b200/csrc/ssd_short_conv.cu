@@ -83,11 +83,12 @@ conv_fwd_kernel(const SsdConvArgs a, const ConvDims d) {
         for (int t = s.t0; t < s.t1; ++t) store_f<VECTOR>(out + static_cast<long long>(t) * a.channels, zero, n);
         return;
     }
-    const T* x = static_cast<const T*>(a.x) + token_row(d.map, s, a.batch_stride, a.token_stride, 0) + c;
+    const Rows<T> x(static_cast<const T*>(a.x) + token_row(d.map, s, a.batch_stride, a.token_stride, 0) + c, a.token_stride);
+    const Rows<T> outs(out, a.channels);
     Pack<T, V> next[kConvAhead];
     const auto request = [&](int t) {
 #pragma unroll
-        for (int i = 0; i < kConvAhead; ++i) load_raw<VECTOR, false>(next[i], x + (t + i) * a.token_stride, t + i < s.t1 ? n : 0);
+        for (int i = 0; i < kConvAhead; ++i) load_raw<VECTOR, false>(next[i], x.at(t + i), t + i < s.t1 ? n : 0);
     };
     request(s.t0);
     Filter<T, V, W> f;
@@ -114,7 +115,7 @@ conv_fwd_kernel(const SsdConvArgs a, const ConvDims d) {
                 for (int k = 0; k < W; ++k) p = fmaf(f.w[k][j], held[k][j], p);
                 o[j] = a.silu ? p * sigmoid_fast(p) : p;
             }
-            if (t + i < s.t1) store_f<VECTOR>(out + static_cast<long long>(t + i) * a.channels, o, n);
+            store_f<VECTOR>(outs.to(t + i), o, t + i < s.t1 ? n : 0);
         }
     }
     if (s.last && a.final_state != nullptr) {
@@ -160,7 +161,8 @@ conv_bwd_kernel(const SsdConvGradArgs g, const ConvDims d, int slices) {
             for (int t = s.t0; t < s.t1; ++t) store_f<VECTOR>(dx + static_cast<long long>(t) * a.channels, zero, n);
             continue;
         }
-        const T* x = static_cast<const T*>(a.x) + token_row(d.map, s, a.batch_stride, a.token_stride, 0) + c;
+        const Rows<T> x(static_cast<const T*>(a.x) + token_row(d.map, s, a.batch_stride, a.token_stride, 0) + c, a.token_stride);
+        const Rows<T> douts(dout, a.channels), dxs(dx, a.channels);
         float held[W][V], dpre[W][V];
 #pragma unroll
         for (int k = 1; k < W; ++k) {
@@ -174,8 +176,8 @@ conv_bwd_kernel(const SsdConvGradArgs g, const ConvDims d, int slices) {
 #pragma unroll
             for (int i = 0; i < kConvAhead; ++i) {
                 const int in = t + i < end ? n : 0;
-                load_raw<VECTOR, false>(xn[i], x + (t + i) * a.token_stride, in);
-                load_raw<VECTOR, false>(dn[i], dout + static_cast<long long>(t + i) * a.channels, in);
+                load_raw<VECTOR, false>(xn[i], x.at(t + i), in);
+                load_raw<VECTOR, false>(dn[i], douts.at(t + i), in);
             }
         };
         request(s.t0);
@@ -227,7 +229,7 @@ conv_bwd_kernel(const SsdConvGradArgs g, const ConvDims d, int slices) {
                     for (int j = 0; j < V; ++j) o[j] += df[j];
                 }
                 if (to >= 0)
-                    store_f<VECTOR>(dx + static_cast<long long>(to) * a.channels, o, n);
+                    store_f<VECTOR>(dxs.to(to), o, n);
                 else if (g.dinitial != nullptr)
                     store_f<VECTOR>(static_cast<T*>(g.dinitial) +
                                         (static_cast<long long>(s.seq) * (W - 1) + (to + W - 1)) * a.channels + c, o, n);
@@ -341,7 +343,7 @@ int conv_check(const SsdConvArgs& a) {
         a.token_stride < 0)
         return SSD_ERR_SHAPE;
     if (a.width < 2 || a.width > 4) return SSD_ERR_UNSUPPORTED;
-    if (a.tokens > 0x7fffffff - (1 << 20) || a.rows > 0x7ffffff0) return SSD_ERR_RANGE;
+    if (a.tokens > 0x7fffffff - (1 << 20) || a.rows > 0x7ffffff0 || !row_steps(a.token_stride, a.channels)) return SSD_ERR_RANGE;
     if ((a.tokens > 0 && !a.x) || !a.weight) return SSD_ERR_NULL;
     return SSD_OK;
 }

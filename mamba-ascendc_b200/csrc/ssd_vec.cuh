@@ -191,6 +191,23 @@ __device__ __forceinline__ long long token_row(const SeqMap& m, const Span& s, l
     return (m.cu == nullptr ? s.seq * batch_stride : 0) + (s.origin + t) * token_stride;
 }
 
+// Rows at a distance that fits 31 bits in bytes (the entry points refuse others), so that a row's address is one multiply-add.
+template <class T>
+struct Rows {
+    const char* base;
+    int step;
+    __device__ __forceinline__ Rows(const T* first, int64_t elements)
+        : base(reinterpret_cast<const char*>(first)), step(static_cast<int>(elements) * static_cast<int>(sizeof(T))) {}
+    __device__ __forceinline__ const T* at(int t) const {
+        return reinterpret_cast<const T*>(base + static_cast<long long>(t) * step);
+    }
+    __device__ __forceinline__ T* to(int t) const { return const_cast<T*>(at(t)); }
+};
+template <class... S>
+inline bool row_steps(S... elements) {
+    return ((elements >= 0 && elements < (1 << 29)) && ...);
+}
+
 // ---- sums over the rows of a table [rows][cols] in a fixed order: the second half of gradients of parameters.
 // Cell (r, c) of `out` gets the sum of column `col`; StoreCol(col, sum) writes it.
 constexpr int kSumCols = 32, kSumRows = 32;
