@@ -3,16 +3,18 @@
 //   g_t = C_t dy_t + a_{t+1} g_{t+1} ;  dC_t[n] = sum_c dy_t h_t[n] ;  dB_t[n] = sum_c g_t[n] dt_t x_t ;  du_t = sum_n g_t[n] B_t[n]
 //   q_t[n] = g_t[n] a_t[n] h_{t-1}[n] ;  ddt_t = x_t du_t + sum_n q_t[n] A[n] ;  dA[n] = sum_t q_t[n] dt_t ;  dx_t = dt_t du_t + D dy_t
 //
-// What bounds it: about 15 instructions for each (token, channel, state column), a fifth of them the sums of dB and dC over
-// the channels, which lie along the lanes.  The bytes are few beside that.
+// What bounds it: instructions, 16 for the arithmetic of each (token, channel, state column) and about ten more: the sums of
+// dB and dC over the channels, which lie along the lanes, the exchange between the warps of a chunk, and what each (token,
+// channel) takes.  The bytes are few beside that.
 //
-// Layout: a lane owns two neighbouring channels (packed arithmetic), a warp kTokens tokens of 64 channels, a CTA a chunk
-// of kWarps * kTokens tokens, which it walks from the sequence's end.  For one state column at a time each warp forms its
-// exponentials once, runs the recurrences of h and g from zero over its tokens, and puts their ends and the product of its
-// decays into shared memory; after one barrier it folds those of the warps before (behind) it into its true start, and
-// runs both recurrences again on the exponentials it still holds.  h enters a chunk from the forward pass's checkpoints, g
-// from the chunk behind.  Sums over n stay with the thread.  dB and dC replace B and C in shared memory (a warp's tokens are
-// its own) and leave as one table per block of channels, summed in a fixed order by scan_shared_sum_kernel.
+// Layout: a lane owns two neighbouring channels, a warp kTokens tokens of 64 channels, a CTA a chunk of kWarps * kTokens tokens,
+// which it walks from the sequence's end.  For one state column at a time each warp forms its exponentials once, runs the
+// recurrences of h and g from zero over its tokens, and puts their ends and the product of its decays into shared memory;
+// after one barrier it folds those of the warps before (behind) it into its true start, and runs both recurrences again on
+// the exponentials it still holds.  h enters a chunk from the forward pass's checkpoints, g from the chunk behind.  Sums over
+// n stay with the thread; sums over the lanes go through shared memory, 38 instructions for 16 values against 62 with shuffles.
+// dB and dC replace B and C in shared memory (a warp's tokens are its own) and leave as one table per block of channels, summed
+// in a fixed order by scan_shared_sum_kernel.
 #include "ssd_selective.cuh"
 
 namespace ssd {
@@ -33,25 +35,29 @@ struct BwdLaunch {
     long long all_tokens;
 };
 
+constexpr int kValues = 2 * kTokens;  // dB and dC of a warp's tokens
+constexpr int kLaneRow = 32 + 4;      // a value of all lanes, padded so that eight lanes read sixteen of them without conflict
 size_t bwd_smem(int dstate) {
-    return sizeof(float) * (2 * dstate * kRow + 4 * dstate * kBwdChannels + 2 * kWarps * kBwdChannels * (2 + 1 + 1));
+    return sizeof(float) * (2 * dstate * kRow + 3 * dstate * kBwdChannels + 2 * kWarps * 32 * (4 + 4 + 2) + kWarps * kValues * kLaneRow);
 }
 
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
-// Sums over the 32 lanes of 16 values each: a lane ends up with the sum of value `lane / 2` (both of a pair the same).  Each
-// step hands half of the values to the lane on the other side, 8 + 4 + 2 + 1 + 1 exchanges instead of 80.
-__device__ __forceinline__ float sum_lanes16(float (&v)[16], int lane) {
+// Sums over the 32 lanes of 16 values each: lane l returns that of value l / 2.  `rows` is the warp's own.
+__device__ __forceinline__ float sum_lanes(const float (&v)[kValues], float* rows, int lane) {
+    __syncwarp();
 #pragma unroll
-    for (int half = 8, bit = 16; half > 0; half >>= 1, bit >>= 1) {
-        const bool upper = (lane & bit) != 0;
+    for (int j = 0; j < kValues; ++j) rows[j * kLaneRow + lane] = v[j];
+    __syncwarp();
+    const float4* half = reinterpret_cast<const float4*>(rows + (lane >> 1) * kLaneRow + (lane & 1) * 16);
+    float4 sum = half[0];
 #pragma unroll
-        for (int i = 0; i < half; ++i) {
-            const float keep = upper ? v[i + half] : v[i], send = upper ? v[i] : v[i + half];
-            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, bit);
-        }
+    for (int i = 1; i < 4; ++i) {
+        const float4 q = half[i];
+        sum = make_float4(sum.x + q.x, sum.y + q.y, sum.z + q.z, sum.w + q.w);
     }
-    return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
+    const float mine = (sum.x + sum.y) + (sum.z + sum.w);
+    return mine + __shfl_xor_sync(0xffffffffu, mine, 1);
 }
 
 template <class T, bool VECTOR, bool GATED>
@@ -94,19 +100,18 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
 
     float* sb = bwd_smem_;                          // [N][kRow] B, later dB
     float* sc = sb + N * kRow;                      // [N][kRow] C, later dC
-    float* sa = sc + N * kRow;                      // [N][64] A log2(e)
-    float* sg = sa + N * kBwdChannels;              // [2][N][64] gradient of the state behind the chunk
-    float* sda = sg + 2 * N * kBwdChannels;         // [N][64] dA
-    float4* ex_h = reinterpret_cast<float4*>(sda + N * kBwdChannels);                   // [2][warps][32] decay, end of h
-    float2* ex_g = reinterpret_cast<float2*>(ex_h + 2 * kWarps * 32);                   // [2][warps][32] end of g
-    float2* ex_a = ex_g + 2 * kWarps * 32;                                              // [2][warps][32] dA of the warp
+    float2* sa = reinterpret_cast<float2*>(sc + N * kRow);  // [N][32] A log2(e) of the lane's channels
+    float2* sg = sa + N * 32;                       // [N][32] gradient of the state behind the chunk
+    float2* sda = sg + N * 32;                      // [N][32] dA
+    float4* ex_h = reinterpret_cast<float4*>(sda + N * 32);  // [2][warps][32] decay, end of h
+    float4* ex_g = ex_h + 2 * kWarps * 32;                   // [2][warps][32] decay, end of g
+    float2* ex_a = reinterpret_cast<float2*>(ex_g + 2 * kWarps * 32);  // [2][warps][32] dA of the warp
+    float* rows = reinterpret_cast<float*>(ex_a + 2 * kWarps * 32) + w * kValues * kLaneRow;
 
     const int c = cb.first + 2 * lane, pn = max(min(cb.n - 2 * lane, 2), 0);
     for (int i = tid; i < N * kBwdChannels; i += 32 * kWarps) {
         const int n = i / kBwdChannels, ch = i % kBwdChannels;
         const bool in = ch < cb.n;
-        sa[i] = in ? a.A[static_cast<long long>(cb.first + ch) * N + n] * kLog2e : 0.f;
-        sda[i] = 0.f;
         float end = 0.f;
         if (in) {
             if (l.split)
@@ -114,24 +119,31 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
             else if (g.dfinal != nullptr)
                 end = g.dfinal[(static_cast<long long>(s.seq) * a.channels + cb.first + ch) * N + n];
         }
-        sg[i] = end;
+        reinterpret_cast<float*>(sa)[i] = in ? a.A[static_cast<long long>(cb.first + ch) * N + n] * kLog2e : 0.f;
+        reinterpret_cast<float*>(sda)[i] = 0.f;
+        reinterpret_cast<float*>(sg)[i] = end;
     }
     float2 bias = make_float2(0.f, 0.f), skip = bias, dskip = bias, dbias = bias;
     if (a.dt_bias != nullptr) bias = make_float2(pn > 0 ? a.dt_bias[c] : 0.f, pn > 1 ? a.dt_bias[c + 1] : 0.f);
     if (a.D != nullptr) skip = make_float2(pn > 0 ? a.D[c] : 0.f, pn > 1 ? a.D[c + 1] : 0.f);
 
-    const T* x = static_cast<const T*>(a.x) + token_row(l.map, s, a.x_strides[0], a.x_strides[1], 0) + c;
-    const T* dtp = static_cast<const T*>(a.dt) + token_row(l.map, s, a.dt_strides[0], a.dt_strides[1], 0) + c;
-    const T* z = static_cast<const T*>(a.z) + token_row(l.map, s, a.z_strides[0], a.z_strides[1], 0) + c;
-    const T* bm = static_cast<const T*>(a.bm) + token_row(l.map, s, a.b_strides[0], a.b_strides[1], 0) + cb.group * a.b_strides[2];
-    const T* cm = static_cast<const T*>(a.cm) + token_row(l.map, s, a.c_strides[0], a.c_strides[1], 0) + cb.group * a.c_strides[2];
-    const T* dout = static_cast<const T*>(g.dout) + first_token * a.channels + c;
+    const Rows<T> xs(static_cast<const T*>(a.x) + first_row(l.map, s, a.x_strides) + c, a.x_strides[1]);
+    const Rows<T> dts(static_cast<const T*>(a.dt) + first_row(l.map, s, a.dt_strides) + c, a.dt_strides[1]);
+    const Rows<T> zs(static_cast<const T*>(a.z) + first_row(l.map, s, a.z_strides) + c, a.z_strides[1]);
+    const Rows<T> douts(static_cast<const T*>(g.dout) + first_token * a.channels + c, a.channels);
+    const Rows<T> bs(static_cast<const T*>(a.bm) + first_row(l.map, s, a.b_strides) + cb.group * a.b_strides[2], a.b_strides[1]);
+    const Rows<T> cs(static_cast<const T*>(a.cm) + first_row(l.map, s, a.c_strides) + cb.group * a.c_strides[2], a.c_strides[1]);
+    const Rows<float> dbs(db, a.groups * N), dcs(dc, a.groups * N);
+    const long long out0 = first_token * a.channels + c;
+    const Rows<T> dxs(static_cast<T*>(g.dx) + out0, a.channels), ddts(static_cast<T*>(g.ddt) + out0, a.channels);
+    const Rows<T> dzs(static_cast<T*>(g.dz) + out0, a.channels);
     const long long checkpoint0 = l.map.cu == nullptr
                                       ? s.seq * ((l.map.tokens + kScanCheckpoint - 1) / kScanCheckpoint)
                                       : s.origin / kScanCheckpoint + s.seq;
+    // B and C of a chunk: a thread has a token and every fourth quad of columns
+    const int quad_t = tid % kChunk, quads = (N + 3) / 4;
 
     const int chunks = (s.t1 - s.t0 + kChunk - 1) / kChunk;
-    int side = 0;  // of sg
     for (int k = chunks - 1; k >= 0; --k) {
         const int t0 = s.t0 + k * kChunk, tw = t0 + w * kTokens;
         // ---- this warp's tokens
@@ -141,10 +153,22 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
 #pragma unroll
         for (int i = 0; i < kTokens; ++i) {
             const int t = tw + i, n = t < s.t1 ? pn : 0;
-            load_raw<VECTOR, false>(xr[i], x + t * a.x_strides[1], n);
-            load_raw<VECTOR, false>(dr[i], dtp + t * a.dt_strides[1], n);
-            load_raw<VECTOR, false>(gr[i], dout + static_cast<long long>(t) * a.channels, n);
-            if (GATED) load_raw<VECTOR, false>(zr[i], z + t * a.z_strides[1], n);
+            load_raw<VECTOR, false>(xr[i], xs.at(t), n);
+            load_raw<VECTOR, false>(dr[i], dts.at(t), n);
+            load_raw<VECTOR, false>(gr[i], douts.at(t), n);
+            if (GATED) load_raw<VECTOR, false>(zr[i], zs.at(t), n);
+        }
+        for (int q = tid / kChunk; q < quads; q += 32 * kWarps / kChunk) {
+            const int n = q * 4, in = t0 + quad_t < s.t1 ? min(N - n, 4) : 0;
+            Pack<T, 4> br, cr;
+            load_raw<VECTOR, false>(br, bs.at(t0 + quad_t) + n, in);
+            load_raw<VECTOR, false>(cr, cs.at(t0 + quad_t) + n, in);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (VECTOR || n + j < N) {
+                    sb[(n + j) * kRow + quad_t] = to_f(br.v[j]);
+                    sc[(n + j) * kRow + quad_t] = to_f(cr.v[j]);
+                }
         }
 #pragma unroll
         for (int i = 0; i < kTokens; ++i) {
@@ -162,170 +186,172 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
             u[i] = pack2(d.x * xv.x, d.y * xv.y);
             dy[i] = pack2(o.x, o.y);
         }
-        for (int i = tid; i < N * kChunk; i += 32 * kWarps) {
-            const int t = i / N, n = i % N;
-            const bool in = t0 + t < s.t1;
-            sb[n * kRow + t] = in ? to_f(bm[(t0 + t) * a.b_strides[1] + n]) : 0.f;
-            sc[n * kRow + t] = in ? to_f(cm[(t0 + t) * a.c_strides[1] + n]) : 0.f;
-        }
         __syncthreads();
 
         F2 ddt2[kTokens], du[kTokens], y[kTokens];
 #pragma unroll
         for (int i = 0; i < kTokens; ++i) ddt2[i] = du[i] = y[i] = {};
-        const F2 total_dt = pack2(sum_dt.x, sum_dt.y);
         const float* hp = a.checkpoints + (checkpoint0 + t0 / kScanCheckpoint) * N * a.channels + c;
         if (k > 0 && lane < kTokens) {  // the next chunk's rows (the tokens before) into L2
             const int t = tw - kChunk + lane;
-            prefetch_l2(x + t * a.x_strides[1] - 2 * lane);
-            prefetch_l2(dtp + t * a.dt_strides[1] - 2 * lane);
-            prefetch_l2(dout + static_cast<long long>(t) * a.channels - 2 * lane);
-            if (GATED) prefetch_l2(z + t * a.z_strides[1] - 2 * lane);
+            prefetch_l2(xs.at(t) - 2 * lane);
+            prefetch_l2(dts.at(t) - 2 * lane);
+            prefetch_l2(douts.at(t) - 2 * lane);
+            if (GATED) prefetch_l2(zs.at(t) - 2 * lane);
         }
-        Pack<float, 2> h_start;
-        load_raw<VECTOR, false>(h_start, hp, pn);  // the state that the chunk starts from, a column ahead
+        Pack<float, 2> h_start;  // the state that the chunk starts from, a column ahead
+        load_raw<VECTOR, false>(h_start, hp, pn);
+        // of the column: A, g behind the chunk, dA, and this warp's tokens of B and C; and this parity's exchange
+        const float2* an = sa + lane;
+        float2* gn = sg + lane;
+        float2* dan = sda + lane;
+        float* bn = sb + w * kTokens;
+        const int c_off = N * kRow;
+        float4* eh = ex_h + lane;
+        float2* ea = ex_a + lane;
+        constexpr int to_h_g = 2 * kWarps * 32;
+        float2 g_before = make_float2(0.f, 0.f);  // warp 0: gradient of the state before the chunk, of the last column
         for (int n = 0; n < N; ++n) {
-            const int buf = n & 1;
-            const F2 a2 = *reinterpret_cast<const F2*>(sa + n * kBwdChannels + 2 * lane);
+            const float2 a2 = *an;
             F2 hs = pack2(h_start.v[0], h_start.v[1]);
-            if (n + 1 < N) load_raw<VECTOR, false>(h_start, hp + static_cast<long long>(n + 1) * a.channels, pn);
+            hp += a.channels;
+            if (n + 1 < N) load_raw<VECTOR, false>(h_start, hp, pn);
             float bt[kTokens], ct[kTokens];
 #pragma unroll
             for (int i = 0; i < kTokens; i += 4) {
-                *reinterpret_cast<float4*>(bt + i) = *reinterpret_cast<const float4*>(sb + n * kRow + w * kTokens + i);
-                *reinterpret_cast<float4*>(ct + i) = *reinterpret_cast<const float4*>(sc + n * kRow + w * kTokens + i);
+                *reinterpret_cast<float4*>(bt + i) = *reinterpret_cast<const float4*>(bn + i);
+                *reinterpret_cast<float4*>(ct + i) = *reinterpret_cast<const float4*>(bn + c_off + i);
             }
             F2 al[kTokens], h[kTokens];
             F2 end_h = {}, end_g = {};
 #pragma unroll
             for (int i = 0; i < kTokens; ++i) {
-                al[i] = exp2_2(mul2(dt[i], a2));
-                h[i] = mul2(u[i], pack2(bt[i], bt[i]));
+                al[i] = pack2(ex2f(dt[i].x * a2.x), ex2f(dt[i].y * a2.y));
+                h[i] = pack2(u[i].x * bt[i], u[i].y * bt[i]);
                 end_h = fma2(al[i], end_h, h[i]);
             }
 #pragma unroll
-            for (int i = kTokens - 1; i >= 0; --i) end_g = mul2(al[i], fma2(pack2(ct[i], ct[i]), dy[i], end_g));
+            for (int i = kTokens - 1; i >= 0; --i)
+                end_g = pack2(al[i].x * fmaf(ct[i], dy[i].x, end_g.x), al[i].y * fmaf(ct[i], dy[i].y, end_g.y));
             {
-                const float2 p = unpack2(exp2_2(mul2(total_dt, a2))), e = unpack2(end_h);
-                ex_h[(buf * kWarps + w) * 32 + lane] = make_float4(p.x, p.y, e.x, e.y);
-                ex_g[(buf * kWarps + w) * 32 + lane] = unpack2(end_g);
+                const float px = ex2f(sum_dt.x * a2.x), py = ex2f(sum_dt.y * a2.y);
+                eh[w * 32] = make_float4(px, py, end_h.x, end_h.y);
+                eh[to_h_g + w * 32] = make_float4(px, py, end_g.x, end_g.y);
             }
             __syncthreads();
-            // dA of the column before, left by all warps before this barrier: one of them adds it up
-            if (n > 0 && w == ((n - 1) & (kWarps - 1))) {
-                float2* at = reinterpret_cast<float2*>(sda + (n - 1) * kBwdChannels + 2 * lane);
-                float2 sum = *at;
+            // what all warps left of the column before: one of them adds up its dA, warp 0 moves its g on
+            if (n > 0) {
+                if (w == ((n - 1) & (kWarps - 1))) {
+                    float2 sum = dan[-32];
+                    const float2* last = ex_a + lane + (((n - 1) & 1) ? kWarps * 32 : 0);
 #pragma unroll
-                for (int v = 0; v < kWarps; ++v) {
-                    const float2 d = ex_a[((buf ^ 1) * kWarps + v) * 32 + lane];
-                    sum = make_float2(sum.x + d.x, sum.y + d.y);
+                    for (int v = 0; v < kWarps; ++v) sum = make_float2(sum.x + last[v * 32].x, sum.y + last[v * 32].y);
+                    dan[-32] = sum;
                 }
-                *at = sum;
+                if (w == 0) gn[-32] = g_before;
             }
-            // all of them loaded at once; whether a warp lies before or behind is the same for all lanes
-            F2 gs = *reinterpret_cast<const F2*>(sg + (side * N + n) * kBwdChannels + 2 * lane);
-            F2 decay[kWarps], end[kWarps];
+            // all loaded at once; whether a warp lies before or behind is the same for all lanes
+            F2 gs = pack2(gn->x, gn->y);
+            float4 e[kWarps];
 #pragma unroll
-            for (int v = 0; v < kWarps; ++v) {
-                const F2* before = reinterpret_cast<const F2*>(ex_h + (buf * kWarps + v) * 32 + lane);
-                const F2* behind = reinterpret_cast<const F2*>(ex_g + (buf * kWarps + v) * 32 + lane);
-                decay[v] = *before;
-                end[v] = v < w ? before[1] : *behind;
-            }
+            for (int v = 0; v < kWarps; ++v)
+                e[v] = eh[(v < w ? 0 : to_h_g) + v * 32];
 #pragma unroll
             for (int v = 0; v < kWarps - 1; ++v)
-                if (v < w) hs = fma2(decay[v], hs, end[v]);
+                if (v < w) hs = pack2(fmaf(e[v].x, hs.x, e[v].z), fmaf(e[v].y, hs.y, e[v].w));
 #pragma unroll
             for (int v = kWarps - 1; v > 0; --v)
-                if (v > w) gs = fma2(decay[v], gs, end[v]);
-            if (w == 0) {
-                *reinterpret_cast<F2*>(sg + ((side ^ 1) * N + n) * kBwdChannels + 2 * lane) = fma2(decay[0], gs, end_g);
-            }
-            float v16[16];  // dB, dC of the tokens, over this lane's channels
+                if (v > w) gs = pack2(fmaf(e[v].x, gs.x, e[v].z), fmaf(e[v].y, gs.y, e[v].w));
+            float v16[kValues];  // dB, dC of the tokens, over this lane's channels
             {
                 F2 prev = hs;
 #pragma unroll
                 for (int i = 0; i < kTokens; ++i) {
                     prev = fma2(al[i], prev, h[i]);
                     h[i] = prev;
-                    v16[8 + i] = sum2(mul2(dy[i], prev));
-                    if (GATED) y[i] = fma2(pack2(ct[i], ct[i]), prev, y[i]);
+                    v16[kTokens + i] = fmaf(dy[i].y, prev.y, dy[i].x * prev.x);
+                    if (GATED) y[i] = pack2(fmaf(ct[i], prev.x, y[i].x), fmaf(ct[i], prev.y, y[i].y));
                 }
             }
             F2 da = {};
 #pragma unroll
             for (int i = kTokens - 1; i >= 0; --i) {
-                const F2 gt = fma2(pack2(ct[i], ct[i]), dy[i], gs);
-                v16[i] = sum2(mul2(gt, u[i]));
-                du[i] = fma2(gt, pack2(bt[i], bt[i]), du[i]);
+                const F2 gt = pack2(fmaf(ct[i], dy[i].x, gs.x), fmaf(ct[i], dy[i].y, gs.y));
+                v16[i] = fmaf(gt.y, u[i].y, gt.x * u[i].x);
+                du[i] = pack2(fmaf(gt.x, bt[i], du[i].x), fmaf(gt.y, bt[i], du[i].y));
                 gs = mul2(gt, al[i]);
                 const F2 q = mul2(gs, i > 0 ? h[i > 0 ? i - 1 : 0] : hs);
-                ddt2[i] = fma2(q, a2, ddt2[i]);
+                ddt2[i] = pack2(fmaf(q.x, a2.x, ddt2[i].x), fmaf(q.y, a2.y, ddt2[i].y));
                 da = fma2(q, dt[i], da);
             }
-            ex_a[(buf * kWarps + w) * 32 + lane] = unpack2(da);
-            const float r = sum_lanes16(v16, lane);
+            g_before = make_float2(gs.x, gs.y);
+            ea[w * 32] = make_float2(da.x, da.y);
+            const float r = sum_lanes(v16, rows, lane);
             // value lane / 2: dB of tokens 0..7, then dC; this warp alone reads these places
-            if ((lane & 1) == 0) (lane < 16 ? sb : sc)[n * kRow + w * kTokens + ((lane >> 1) & 7)] = r;
+            if ((lane & 1) == 0) bn[(lane < 16 ? 0 : c_off) + ((lane >> 1) & 7)] = r;
+            an += 32;
+            gn += 32;
+            dan += 32;
+            bn += kRow;
+            // the other parity
+            eh += n % 2 == 0 ? kWarps * 32 : -kWarps * 32;
+            ea += n % 2 == 0 ? kWarps * 32 : -kWarps * 32;
         }
         __syncthreads();
         if (w == ((N - 1) & (kWarps - 1))) {
-            float2* at = reinterpret_cast<float2*>(sda + (N - 1) * kBwdChannels + 2 * lane);
-            float2 sum = *at;
+            float2 sum = dan[-32];
+            const float2* last = ex_a + lane + (((N - 1) & 1) ? kWarps * 32 : 0);
 #pragma unroll
-            for (int v = 0; v < kWarps; ++v) {
-                const float2 d = ex_a[(((N - 1) & 1) * kWarps + v) * 32 + lane];
-                sum = make_float2(sum.x + d.x, sum.y + d.y);
-            }
-            *at = sum;
+            for (int v = 0; v < kWarps; ++v) sum = make_float2(sum.x + last[v * 32].x, sum.y + last[v * 32].y);
+            dan[-32] = sum;
         }
-        for (int i = tid; i < N * kChunk; i += 32 * kWarps) {
-            const int t = i / N, n = i % N;
-            if (t0 + t < s.t1) {
-                const long long at = static_cast<long long>(t0 + t) * a.groups * N + n;
-                db[at] = sb[n * kRow + t];
-                dc[at] = sc[n * kRow + t];
+        if (w == 0) gn[-32] = g_before;
+        if (t0 + quad_t < s.t1) {
+            for (int q = tid / kChunk; q < quads; q += 32 * kWarps / kChunk) {
+                const int n = q * 4;
+                float fb[4], fc[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (VECTOR || n + j < N) fb[j] = sb[(n + j) * kRow + quad_t], fc[j] = sc[(n + j) * kRow + quad_t];
+                store_f<VECTOR>(dbs.to(t0 + quad_t) + n, fb, min(N - n, 4));
+                store_f<VECTOR>(dcs.to(t0 + quad_t) + n, fc, min(N - n, 4));
             }
         }
 #pragma unroll
         for (int i = 0; i < kTokens; ++i) {
             const int t = tw + i, n = t < s.t1 ? pn : 0;
-            load_raw<VECTOR, false>(xr[i], x + t * a.x_strides[1], n);
-            load_raw<VECTOR, false>(dr[i], dtp + t * a.dt_strides[1], n);
+            load_raw<VECTOR, false>(xr[i], xs.at(t), n);
+            load_raw<VECTOR, false>(dr[i], dts.at(t), n);
             if (GATED) {
-                load_raw<VECTOR, false>(zr[i], z + t * a.z_strides[1], n);
-                load_raw<VECTOR, false>(gr[i], dout + static_cast<long long>(t) * a.channels, n);
+                load_raw<VECTOR, false>(zr[i], zs.at(t), n);
+                load_raw<VECTOR, false>(gr[i], douts.at(t), n);
             }
         }
 #pragma unroll
         for (int i = 0; i < kTokens; ++i) {
             const int t = tw + i, n = t < s.t1 ? pn : 0;
             const float2 xv = pair_f(xr[i]);
-            const float2 dv = unpack2(dt[i]), duv = unpack2(du[i]), dyv = unpack2(dy[i]), qa = unpack2(ddt2[i]);
             constexpr float kLn2 = 0.6931471805599453f;
-            float2 dd = make_float2(fmaf(qa.x, kLn2, xv.x * duv.x), fmaf(qa.y, kLn2, xv.y * duv.y));
+            float2 dd = make_float2(fmaf(ddt2[i].x, kLn2, xv.x * du[i].x), fmaf(ddt2[i].y, kLn2, xv.y * du[i].y));
             if (a.softplus) {
                 const float2 raw = pair_f(dr[i]);
                 dd.x *= sigmoid_fast(raw.x + bias.x);
                 dd.y *= sigmoid_fast(raw.y + bias.y);
             }
-            const long long at = (first_token + t) * a.channels + c;
-            store_pair<VECTOR>(static_cast<T*>(g.dx) + at,
-                               make_float2(fmaf(dv.x, duv.x, skip.x * dyv.x), fmaf(dv.y, duv.y, skip.y * dyv.y)), n);
-            store_pair<VECTOR>(static_cast<T*>(g.ddt) + at, dd, n);
+            store_pair<VECTOR>(dxs.to(t), make_float2(fmaf(dt[i].x, du[i].x, skip.x * dy[i].x), fmaf(dt[i].y, du[i].y, skip.y * dy[i].y)),
+                               n);
+            store_pair<VECTOR>(ddts.to(t), dd, n);
             if (GATED) {
-                const float2 zv = pair_f(zr[i]), yv = unpack2(y[i]), o = pair_f(gr[i]);
+                const float2 zv = pair_f(zr[i]), o = pair_f(gr[i]);
                 const float gx = sigmoid_fast(zv.x), gy = sigmoid_fast(zv.y);
-                store_pair<VECTOR>(static_cast<T*>(g.dz) + at,
-                                   make_float2(o.x * fmaf(skip.x, xv.x, yv.x) * gx * fmaf(zv.x, 1.f - gx, 1.f),
-                                               o.y * fmaf(skip.y, xv.y, yv.y) * gy * fmaf(zv.y, 1.f - gy, 1.f)), n);
+                store_pair<VECTOR>(dzs.to(t), make_float2(o.x * fmaf(skip.x, xv.x, y[i].x) * gx * fmaf(zv.x, 1.f - gx, 1.f),
+                                                          o.y * fmaf(skip.y, xv.y, y[i].y) * gy * fmaf(zv.y, 1.f - gy, 1.f)), n);
             }
             if (n > 0) {
-                dskip = make_float2(fmaf(dyv.x, xv.x, dskip.x), fmaf(dyv.y, xv.y, dskip.y));
+                dskip = make_float2(fmaf(dy[i].x, xv.x, dskip.x), fmaf(dy[i].y, xv.y, dskip.y));
                 dbias = make_float2(dbias.x + dd.x, dbias.y + dd.y);
             }
         }
-        side ^= 1;
         __syncthreads();  // before B and C of the next chunk
     }
 
@@ -340,7 +366,7 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
         if (ch >= cb.n) continue;
         float v = 0.f;
         if (n < N) {
-            v = sda[i];
+            v = reinterpret_cast<const float*>(sda)[i];
         } else {
             const float* part = reinterpret_cast<const float*>(ex + (n == N ? 0 : kWarps) * 32);
             for (int k = 0; k < kWarps; ++k) v += part[k * kBwdChannels + ch];
@@ -348,7 +374,7 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
         row[static_cast<long long>(n) * a.channels + ch] = v;
         if (n < N && s.first && g.dinitial != nullptr)
             g.dinitial[(static_cast<long long>(s.seq) * a.channels + cb.first + ch) * N + n] =
-                sg[(side * N + n) * kBwdChannels + ch];
+                reinterpret_cast<const float*>(sg)[i];
     }
 }
 
@@ -391,7 +417,7 @@ BwdSizes bwd_sizes(const SsdScanArgs& a) {
     z.segments = scan_segments(a, kBwdChannels, sm_count());
     z.blocks = scan_blocks(a.channels, a.groups, kBwdChannels);
     z.all_tokens = a.cu_seqlens ? a.tokens : a.tokens * a.rows;
-    z.ends = scan_segment_floats(a, z.segments);
+    z.ends = (scan_segment_floats(a, z.segments) + 3) / 4 * 4;  // the tables behind are written four floats at a time
     z.shared = 2 * static_cast<size_t>(z.blocks.per_group) * z.all_tokens * a.groups * a.dstate;
     z.channel = static_cast<size_t>(z.segments.items) * (a.dstate + 2) * a.channels;
     return z;

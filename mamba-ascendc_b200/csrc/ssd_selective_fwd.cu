@@ -373,7 +373,9 @@ int scan_check(const SsdScanArgs& a) {
         return SSD_ERR_SHAPE;
     if (a.dstate > kScanMaxState || a.dtype < SSD_F32 || a.dtype > SSD_F16) return SSD_ERR_UNSUPPORTED;
     if (a.tokens > 0x7fffffff - (1 << 20) || a.rows > 0x7ffffff0) return SSD_ERR_RANGE;
-    if (!row_steps(a.x_strides[1], a.dt_strides[1], a.z_strides[1], a.b_strides[1], a.c_strides[1], a.channels)) return SSD_ERR_RANGE;
+    if (!row_steps(a.x_strides[1], a.dt_strides[1], a.z_strides[1], a.b_strides[1], a.c_strides[1], a.channels,
+                   static_cast<int64_t>(a.groups) * a.dstate))
+        return SSD_ERR_RANGE;
     if (!a.A || (a.tokens > 0 && (!a.x || !a.dt || !a.bm || !a.cm))) return SSD_ERR_NULL;
     return SSD_OK;
 }
