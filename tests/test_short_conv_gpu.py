@@ -285,3 +285,21 @@ def test_captured_step_reads_the_slots_of_each_replay():
         torch.cuda.synchronize()
         eager = kept.clone()
         assert torch.equal(out, ak.short_conv_step(x, eager, weight, bias, "silu", slots)) and torch.equal(state, eager)
+
+
+def test_gradients_cannot_be_differentiated_again():
+    x, weight, bias, initial = make(1, 9, 8, 4, torch.float32)
+    leaves = [t.requires_grad_(True) for t in (x, weight, bias, initial)]
+    dout = torch.randn_like(x).requires_grad_(True)
+    grads = torch.autograd.grad(ak.short_conv(*leaves[:3], "silu", leaves[3]), leaves, dout, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        grads[0].sum().backward()
+
+
+def test_saved_tensors_that_change_are_an_error():
+    x, weight, bias, initial = make(1, 9, 8, 4, torch.float32)
+    weight.requires_grad_(True)
+    out = ak.short_conv(x, weight, bias, "silu", initial)
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out.sum(), weight)
