@@ -40,6 +40,13 @@ __device__ __forceinline__ float softplus_series(float v) {
     return fmaf(p, s, fmaxf(v, 0.f));
 }
 
+// A in powers of two.  Minus infinity (a column that keeps nothing) becomes the lowest number that a step of zero, as tokens
+// behind the end of a sequence have it, turns into zero and not into NaN.
+__device__ __forceinline__ float decay_rate(float a) {
+    const float v = a * kLog2e;
+    return v == -INFINITY ? -3.0e38f : v;
+}
+
 // The channels of a CTA lie in one group.
 struct ScanBlocks {
     int per_cta, per_group;  // channels of a CTA, CTAs of a group

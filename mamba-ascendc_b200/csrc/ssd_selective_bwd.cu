@@ -119,7 +119,7 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
             else if (g.dfinal != nullptr)
                 end = g.dfinal[(static_cast<long long>(s.seq) * a.channels + cb.first + ch) * N + n];
         }
-        reinterpret_cast<float*>(sa)[i] = in ? a.A[static_cast<long long>(cb.first + ch) * N + n] * kLog2e : 0.f;
+        reinterpret_cast<float*>(sa)[i] = in ? decay_rate(a.A[static_cast<long long>(cb.first + ch) * N + n]) : 0.f;
         reinterpret_cast<float*>(sda)[i] = 0.f;
         reinterpret_cast<float*>(sg)[i] = end;
     }

@@ -76,7 +76,7 @@ selective_walk_kernel(const SsdScanArgs a, const ScanLaunch l) {
     for (int j = 0; j < NPL; ++j) {
         const int n = n0 + j;
         const bool in = live && n < a.dstate;
-        a2[j] = in ? a.A[static_cast<long long>(c) * a.dstate + n] * kLog2e : 0.f;
+        a2[j] = in ? decay_rate(a.A[static_cast<long long>(c) * a.dstate + n]) : 0.f;
         h[j] = 0.f;
         if (kMode == kForward && in) {
             if (l.split)
@@ -317,7 +317,7 @@ selective_join_kernel(const SsdScanArgs a, const SeqMap map, float* work, const 
         count = max((len + map.span - 1) / map.span, 1LL);
     }
     const float* sums = work + map.items() * per;
-    const float a2 = a.A[static_cast<long long>(c) * a.dstate + n] * kLog2e;
+    const float a2 = decay_rate(a.A[static_cast<long long>(c) * a.dstate + n]);
     float v = outer != nullptr ? outer[(static_cast<long long>(seq) * a.channels + c) * a.dstate + n] : 0.f;
     for (long long k = 0; k < count; ++k) {
         const long long item = first + (REVERSE ? count - 1 - k : k);

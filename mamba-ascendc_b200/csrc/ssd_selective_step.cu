@@ -98,7 +98,7 @@ selective_step_kernel(const SsdScanStepArgs a, const ScanBlocks b) {
         if (row0 + k / (2 * kWide) < a.rows) stage_shared(k / (2 * kWide), row0 + k / (2 * kWide), k % (2 * kWide));
     load_state(a2, a.A + own, true);
 #pragma unroll
-    for (int j = 0; j < kStepCols; ++j) a2[j] *= kLog2e;
+    for (int j = 0; j < kStepCols; ++j) a2[j] = decay_rate(a2[j]);
     __syncthreads();
     unsigned found = 0;
     if (a.slots != nullptr) {

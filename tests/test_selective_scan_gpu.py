@@ -420,3 +420,100 @@ def test_a_prompt_and_then_tokens_are_one_sequence():
     top, top_h = magnitudes(*tensors[:8], True, initial)
     near(torch.cat([first, torch.stack(rest, 1)], 1), whole.double(), top, rounding_count(40))
     near(state, end.double(), top_h, rounding_count(40))
+
+
+def test_columns_that_keep_nothing():
+    """A = -inf: such a column is the last token's own contribution; lengths that end inside a tile, and inside a chunk."""
+    for l in (5, 33, 70):
+        x, dt, A, B, C, D, z, bias, initial = make(1, l, 40, 16, 1, torch.float32)
+        A[::3, 2] = float("-inf")
+        A[1] = float("-inf")
+        leaves = [t.detach().requires_grad_(True) for t in (x, dt, A, B, C, D, z, bias, initial)]
+        out, final = ak.selective_scan(*leaves[:8], True, leaves[8], return_final_state=True)
+        want, last = scan_plain(*map(double, (x, dt, A, B, C, D, z, bias)), True, double(initial))
+        top, top_h = magnitudes(x, dt, A, B, C, D, z, bias, True, initial)
+        near(out.detach(), want, top, rounding_count(l), flushed=flush(l))
+        near(final.detach(), last, top_h, rounding_count(l), flushed=flush(l))
+        for g in torch.autograd.grad([out, final], leaves, [torch.ones_like(out), torch.ones_like(final)]):
+            assert g.isfinite().all()
+        state = initial.clone()
+        arguments, options = step_inputs([t[:, :1] if i in (0, 1, 3, 4, 6) else t for i, t in enumerate(
+            (x, dt, A, B, C, D, z, bias, initial))])
+        ak.selective_scan_step(*arguments, state, **options)
+        assert state.isfinite().all()
+
+
+def test_what_lies_behind_or_in_other_sequences_does_not_spread():
+    """Infinities and NaN behind the last packed sequence, in a neighbouring sequence and in rows of padding."""
+    lengths, c, n = [20, 45, 30], 36, 16
+    total = sum(lengths) + 9
+    tensors = make(1, total, c, n, 1, torch.float32, states=3)
+    cu = torch.tensor([0] + lengths).cumsum(0).to("cuda", torch.int32)
+    spoilt = [t.clone() for t in tensors]
+    for i in (0, 1, 3, 4, 6):
+        spoilt[i][:, sum(lengths):] = float("nan")
+        spoilt[i][:, 20:65] = float("inf")
+    results = []
+    for ts in (tensors, spoilt):
+        leaves = [t.detach().requires_grad_(True) for t in ts]
+        out, final = ak.selective_scan(*leaves[:8], True, leaves[8], cu, True)
+        dout = torch.ones_like(out)
+        dout[:, sum(lengths):] = float("nan")
+        grads = torch.autograd.grad([out, final], [leaves[i] for i in (0, 1, 3, 4, 6)], [dout, torch.ones_like(final)])
+        results.append([out.detach(), *grads])
+        states = final.detach()[[0, 2]]
+        results[-1].append(states)
+    for good, bad in zip(*results):
+        if good.shape[1] == total:
+            for own in (slice(0, 20), slice(65, 95), slice(95, total)):
+                assert torch.equal(good[:, own], bad[:, own])
+        else:
+            assert torch.equal(good, bad)
+    step = make(4, 1, c, n, 1, torch.float32, start=False)
+    step[0][2] = float("nan")
+    arguments, options = step_inputs(step)
+    state = torch.randn(6, c, n, device="cuda")
+    state[5] = float("nan")
+    out = ak.selective_scan_step(*arguments, state, **options, slots=torch.tensor([1, 0, -1, 3], dtype=torch.int32, device="cuda"))
+    assert out.isfinite().all() and not out[2].any() and state[:5].isfinite().all() and state[5].isnan().all()
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements in the activations, and in a cache of states; what lies at their end equals the same alone."""
+    c, n, tail = 4096, 4, 96
+    total = 2 ** 31 // c + 1000
+    x = torch.zeros(1, total, c, device="cuda", dtype=torch.bfloat16)
+    B, C = (torch.randn(1, total, 1, n, device="cuda").to(torch.bfloat16) for _ in range(2))
+    x[:, -tail:] = torch.randn(1, tail, c, device="cuda").to(torch.bfloat16)
+    A = -torch.rand(c, n, device="cuda")
+    cu = torch.tensor([0, total - tail, total], dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        out, final = ak.selective_scan(x, x, A, B, C, dt_softplus=True, cu_seqlens=cu, return_final_state=True)
+        end = [t[:, -tail:].contiguous() for t in (x, B, C)]
+        want, last = ak.selective_scan(end[0], end[0], A, end[1], end[2], dt_softplus=True, return_final_state=True)
+        top, top_h = magnitudes(end[0], end[0], A, end[1], end[2], None, None, None, True, None)
+        near(out[:, -tail:], want.double(), top, 2 * rounding_count(tail))
+        near(final[1:], last.double(), top_h, 2 * rounding_count(tail))
+        assert not out[:, :-tail].any()
+        del out
+        weight = torch.randn(c, 4, device="cuda")
+        conv, held = ak.short_conv(x, weight, None, "silu", None, cu, True)
+        alone, ends = ak.short_conv(end[0], weight, None, "silu", return_final_state=True)
+        assert torch.equal(conv[:, -tail:], alone) and torch.equal(held[1:], ends)
+        del conv
+        # how a row's squares are added up depends on the number of rows: a value may fall on the other side of a border
+        # between two numbers of the type, one step away (2^-7 of it in bf16, 2^-3 in e4m3)
+        ones = torch.ones(c, device="cuda")
+        for f, step in ((lambda t: ak.rms_norm(t, ones), 2.0 ** -7), (lambda t: ak.rms_norm_quant(t, ones)[0], 2.0 ** -3)):
+            there, here = f(x)[:, -tail:].float(), f(end[0]).float()
+            assert ((there - here).abs() <= step * torch.maximum(there.abs(), here.abs())).all() and here.any(-1).all()
+        del x
+        wide = 128
+        slots = 2 ** 31 // (c * wide) + 3
+        cache = torch.empty(slots, c, wide, device="cuda")
+        cache[-1] = torch.randn(c, wide, device="cuda")
+        state = cache[-1:].clone()
+        tensors = make(1, 1, c, wide, 1, torch.float32, start=False)
+        arguments, options = step_inputs(tensors)
+        one = ak.selective_scan_step(*arguments, cache, **options, slots=torch.tensor([slots - 1], dtype=torch.int32, device="cuda"))
+        assert torch.equal(one, ak.selective_scan_step(*arguments, state, **options)) and torch.equal(cache[-1:], state)
