@@ -16,11 +16,12 @@ namespace {
 
 constexpr int kNormMaxWidth = 16384;
 constexpr int kNormThreads = 512;
+constexpr long long kNormMaxRows = 0x7fffffff - (1 << 20);  // a walk's step behind the last is still a number
 
 template <class T>
 constexpr int kNormVec = 16 / static_cast<int>(sizeof(T));
 
-// Sums and maxima over the tpr threads of a row; `part` has room for 2 x 32 floats per call site.
+// Sums and maxima over the tpr threads of a row; `part` has room for 2 x 16 floats per call site.
 struct Reduced {
     float sum, top;
 };
@@ -32,16 +33,19 @@ __device__ __forceinline__ Reduced reduce_row(float sum, float top, int tpr, flo
         if (TOP) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
     if (tpr > 32) {  // then the row is the whole CTA's
-        const int warp = threadIdx.x >> 5, warps = tpr >> 5;
-        if ((threadIdx.x & 31) == 0) {
+        const int warp = threadIdx.x >> 5, warps = tpr >> 5, lane = threadIdx.x & 31;
+        if (lane == 0) {
             part[warp] = sum;
-            if (TOP) part[32 + warp] = top;
+            if (TOP) part[16 + warp] = top;
         }
         __syncthreads();
-        sum = 0.f;
-        for (int i = 0; i < warps; ++i) {
-            sum += part[i];
-            if (TOP) top = max_nan(top, part[32 + i]);
+        // at most 16 warps
+        sum = (lane & 15) < warps ? part[lane & 15] : 0.f;
+        if (TOP) top = (lane & 15) < warps ? part[16 + (lane & 15)] : 0.f;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (TOP) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
         }
     }
     return {sum, top};
@@ -53,12 +57,12 @@ template <class T, class R, int ITER, bool VECTOR, NormOut kOut>
 __global__ void __launch_bounds__(kNormThreads)
 norm_fwd_kernel(const SsdNormArgs a, int tpr) {
     constexpr int VEC = kNormVec<T>;
-    __shared__ float part[64];
-    const int at = threadIdx.x % tpr;
-    const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
+    __shared__ float part[32];
+    const int at = tpr == 32 ? threadIdx.x & 31 : threadIdx.x;
+    const int row = tpr == 32 ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     const bool live = row < a.rows;
-    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-    const R* res = static_cast<const R*>(a.residual) + row * a.residual_stride;
+    const T* x = Rows<T>(static_cast<const T*>(a.x), a.x_stride).at(row);
+    const R* res = Rows<R>(static_cast<const R*>(a.residual), a.residual_stride).at(row);
     Pack<T, VEC> xr[ITER];
     Pack<R, VEC> rr[ITER];
 #pragma unroll
@@ -86,7 +90,7 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
             unpack(r, rr[i]);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) v[i][j] += r[j];
-            store_f<VECTOR>(static_cast<R*>(a.stream) + row * a.width + c, v[i], n);
+            store_f<VECTOR>(Rows<R>(static_cast<R*>(a.stream), a.width).to(row) + c, v[i], n);
         }
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
@@ -103,7 +107,7 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
             const int c = (at + i * tpr) * VEC, n = live ? min(a.width - c, VEC) : 0;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) v[i][j] = v[i][j] * rstd * w[i][j];
-            store_f<VECTOR>(static_cast<T*>(a.out) + row * a.width + c, v[i], n);
+            store_f<VECTOR>(Rows<T>(static_cast<T*>(a.out), a.width).to(row) + c, v[i], n);
         }
     } else {
         float scale = 1.f;
@@ -129,7 +133,7 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
                 scale = m * (1.f / 448.f);
                 if (scale == 0.f) scale = 1.f;
                 const int lg = 31 - __clz(a.group);
-                if (n > 0 && (c & (a.group - 1)) == 0) a.scales[row * (a.width >> lg) + (c >> lg)] = scale;
+                if (n > 0 && (c & (a.group - 1)) == 0) a.scales[static_cast<long long>(row) * (a.width >> lg) + (c >> lg)] = scale;
             }
             // times the reciprocal (one step off at most), but for scales so small that it would overflow
             if (fabsf(scale) < 1e-30f) {
@@ -146,7 +150,7 @@ norm_fwd_kernel(const SsdNormArgs a, int tpr) {
                 *reinterpret_cast<unsigned*>(q + j) =
                     __nv_cvt_float2_to_fp8x2(make_float2(y[j], y[j + 1]), __NV_SATFINITE, __NV_E4M3) |
                     static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y[j + 2], y[j + 3]), __NV_SATFINITE, __NV_E4M3)) << 16;
-            unsigned char* dst = static_cast<unsigned char*>(a.q) + row * a.width + c;
+            unsigned char* dst = Rows<unsigned char>(static_cast<unsigned char*>(a.q), a.width).to(row) + c;
             if constexpr (VECTOR) {
                 using B = typename Bits<VEC>::type;
                 if (n > 0) *reinterpret_cast<B*>(dst) = *reinterpret_cast<B*>(q);
@@ -166,9 +170,10 @@ template <class T, class R, int ITER, bool VECTOR>
 __global__ void __launch_bounds__(kNormThreads, ITER == 1 ? 2 : 1)
 norm_bwd_kernel(const SsdNormGradArgs a, int tpr) {
     constexpr int VEC = kNormVec<T>;
-    __shared__ float part[2][64];
+    __shared__ float part[2][32];
     extern __shared__ float norm_rows[];  // [rows of the CTA][width], only where there are several
-    const int at = threadIdx.x % tpr, rows_here = blockDim.x / tpr, mine = threadIdx.x / tpr;
+    const int at = tpr == 32 ? threadIdx.x & 31 : threadIdx.x, mine = tpr == 32 ? threadIdx.x >> 5 : 0;
+    const int rows_here = tpr == 32 ? blockDim.x >> 5 : 1;
     float dw[ITER][VEC];
 #pragma unroll
     for (int i = 0; i < ITER; ++i)
@@ -177,25 +182,29 @@ norm_bwd_kernel(const SsdNormGradArgs a, int tpr) {
     Pack<R, VEC> vr[ITER], sr[ITER];
     Pack<T, VEC> gr[ITER], ur[ITER];
     float rstd_next = 0.f;
-    const auto request = [&](long long row) {
+    const Rows<R> streams(static_cast<const R*>(a.stream), a.stream_stride), dstreams(static_cast<const R*>(a.dstream), a.dstream_stride);
+    const Rows<T> douts(static_cast<const T*>(a.dout), a.dout_stride), addends(static_cast<const T*>(a.addend), a.addend_stride);
+    const Rows<T> dxs(static_cast<T*>(a.dx), a.width);
+    const Rows<R> dresiduals(static_cast<R*>(a.dresidual), a.width);
+    const auto request = [&](int row) {
         const bool live = row < a.rows;
         rstd_next = live ? __ldg(a.rstd + row) : 0.f;
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             const int c = (at + i * tpr) * VEC, n = live ? min(a.width - c, VEC) : 0;
-            load_raw<VECTOR, false>(vr[i], static_cast<const R*>(a.stream) + row * a.stream_stride + c, n);
-            load_raw<VECTOR, false>(gr[i], static_cast<const T*>(a.dout) + row * a.dout_stride + c, n);
+            load_raw<VECTOR, false>(vr[i], streams.at(row) + c, n);
+            load_raw<VECTOR, false>(gr[i], douts.at(row) + c, n);
             if (a.dstream != nullptr)
-                load_raw<VECTOR, false>(sr[i], static_cast<const R*>(a.dstream) + row * a.dstream_stride + c, n);
+                load_raw<VECTOR, false>(sr[i], dstreams.at(row) + c, n);
             if (a.addend != nullptr)
-                load_raw<VECTOR, false>(ur[i], static_cast<const T*>(a.addend) + row * a.addend_stride + c, n);
+                load_raw<VECTOR, false>(ur[i], addends.at(row) + c, n);
         }
     };
-    const long long step = static_cast<long long>(gridDim.x) * rows_here;
-    request(static_cast<long long>(blockIdx.x) * rows_here + mine);
+    const int step = gridDim.x * rows_here, count = static_cast<int>(a.rows);
+    request(blockIdx.x * rows_here + mine);
     int parity = 0;
-    for (long long first = static_cast<long long>(blockIdx.x) * rows_here; first < a.rows; first += step) {
-        const long long row = first + mine;
+    for (int first = blockIdx.x * rows_here; first < count; first += step) {
+        const int row = first + mine;
         const bool live = row < a.rows;
         const float rstd = rstd_next;
         float v[ITER][VEC], g[ITER][VEC];
@@ -226,7 +235,7 @@ norm_bwd_kernel(const SsdNormGradArgs a, int tpr) {
                 dot = fmaf(g[i][j], v[i][j], dot);
             }
         }
-        if (first + step < a.rows) request(row + step);
+        if (first + step < count) request(row + step);
         const float mean = reduce_row<false>(dot, 0.f, tpr, part[parity]).sum / static_cast<float>(a.width);
         parity ^= 1;
 #pragma unroll
@@ -236,8 +245,8 @@ norm_bwd_kernel(const SsdNormGradArgs a, int tpr) {
             if (a.dstream != nullptr) unpack(d, s[i]);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) g[i][j] = fmaf(rstd, fmaf(-v[i][j], mean, g[i][j]), d[j]);
-            store_f<VECTOR>(static_cast<T*>(a.dx) + row * a.width + c, g[i], n);
-            if (a.dresidual != nullptr) store_f<VECTOR>(static_cast<R*>(a.dresidual) + row * a.width + c, g[i], n);
+            store_f<VECTOR>(dxs.to(row) + c, g[i], n);
+            if (a.dresidual != nullptr) store_f<VECTOR>(dresiduals.to(row) + c, g[i], n);
         }
     }
     if (a.dweight == nullptr) return;
@@ -333,6 +342,7 @@ extern "C" int ssd_rms_norm_fwd(const SsdNormArgs* args, ssd_stream_t stream) {
     const SsdNormArgs& a = *args;
     if (a.rows <= 0 || a.width <= 0 || a.x_stride < 0 || a.residual_stride < 0) return SSD_ERR_SHAPE;
     if (a.width > kNormMaxWidth) return SSD_ERR_UNSUPPORTED;
+    if (a.rows > kNormMaxRows || !row_steps(a.x_stride, a.residual_stride)) return SSD_ERR_RANGE;
     const bool quant = a.q != nullptr;
     if (!a.x || !a.weight || (!quant && !a.out) || (a.residual && !a.stream) || (quant && !a.static_scale && !a.scales))
         return SSD_ERR_NULL;
@@ -385,6 +395,7 @@ extern "C" int ssd_rms_norm_bwd(const SsdNormGradArgs* args, ssd_stream_t stream
     if (a.rows <= 0 || a.width <= 0 || a.dout_stride < 0 || a.dstream_stride < 0 || a.stream_stride < 0 ||
         a.addend_stride < 0) return SSD_ERR_SHAPE;
     if (a.width > kNormMaxWidth) return SSD_ERR_UNSUPPORTED;
+    if (a.rows > kNormMaxRows || !row_steps(a.dout_stride, a.dstream_stride, a.stream_stride, a.addend_stride)) return SSD_ERR_RANGE;
     if (!a.dout || !a.stream || !a.weight || !a.rstd || !a.dx || (a.dweight && !a.work)) return SSD_ERR_NULL;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return with_type(a.dtype, [&](auto t) {
