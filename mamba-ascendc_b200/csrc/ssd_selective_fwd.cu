@@ -183,7 +183,7 @@ selective_walk_kernel(const SsdScanArgs a, const ScanLaunch l) {
         // way, and the next one's exponentials lie between the steps of this one's recurrence, all in one straight line.
         // Groups of four or eight tokens take 4 to 10% longer: their loads and exponentials come in bursts.  Rows behind the
         // last token have dt = 0; where they are half of the tile they are left out.
-                constexpr int kGroup = 2, kAhead = NPL <= 2 ? 2 : 1;
+        constexpr int kGroup = 2, kAhead = NPL <= 2 ? 2 : 1;
         struct Operands {
             float dt[kGroup], u[kGroup], b[NPL][kGroup], c[NPL][kGroup];
         };

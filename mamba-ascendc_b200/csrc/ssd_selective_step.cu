@@ -30,7 +30,7 @@ template <class T, int LPC, int ROWS, bool VECTOR>
 __global__ void __launch_bounds__(kStepThreads)
 selective_step_kernel(const SsdScanStepArgs a, const ScanBlocks b) {
     constexpr int kChannels = kStepThreads / LPC, kWide = LPC * kStepCols;  // channels of a CTA, columns with those behind dstate
-    __shared__ unsigned flags;  // bit i: row i's slot is taken by an earlier row; bit 16 + i: a later row names it too
+    __shared__ unsigned flags[kStepThreads / 32];  // see shared_slots
     __shared__ float4 token[ROWS][kChannels];  // dt, dt x, gate, gated skip connection
     __shared__ __align__(16) float shared[ROWS][2][kWide];
     const int row0 = blockIdx.x * ROWS, tid = threadIdx.x;
@@ -88,7 +88,7 @@ selective_step_kernel(const SsdScanStepArgs a, const ScanBlocks b) {
         const int n = k % kWide;
         shared[i][k / kWide][n] = n < a.dstate ? to_f(__ldg((k < kWide ? bs : cs).at(row) + n)) : 0.f;
     };
-    if (tid == 0) flags = 0;
+    shared_slots<ROWS, kStepThreads>(slot, a.slots, a.rows, row0, flags);
     // all threads, whatever the row: a row of padding is staged as its slot would be
 #pragma unroll
     for (int k = tid; k < ROWS * kChannels; k += kStepThreads)
@@ -100,19 +100,7 @@ selective_step_kernel(const SsdScanStepArgs a, const ScanBlocks b) {
 #pragma unroll
     for (int j = 0; j < kStepCols; ++j) a2[j] = decay_rate(a2[j]);
     __syncthreads();
-    unsigned found = 0;
-    if (a.slots != nullptr) {
-        unsigned bits = 0;
-        for (int r = tid; r < a.rows; r += kStepThreads) {
-            const int other = a.slots[r];
-#pragma unroll
-            for (int i = 0; i < ROWS; ++i)
-                if (other == slot[i] && r != row0 + i) bits |= r < row0 + i ? 1u << i : 0x10000u << i;
-        }
-        if (bits != 0) atomicOr(&flags, bits);
-        __syncthreads();
-        found = flags;
-    }
+    const unsigned found = a.slots != nullptr ? any_flag(flags) : 0;
 
     // one token: the state moved on, and its output
     const auto step = [&](float (&s)[kStepCols], int i, int row) {

@@ -266,11 +266,11 @@ conv_dw_kernel(const float* table, long long rows, int channels, int width, void
 template <class T, int V, int W, int ROWS, bool VECTOR>
 __global__ void __launch_bounds__(kConvThreads)
 conv_step_kernel(const SsdConvStepArgs a, int channel_blocks) {
-    __shared__ unsigned flags;  // bit i: row i's slot is taken by an earlier row; bit 16 + i: a later row names it too
+    __shared__ unsigned flags[kConvThreads / 32];  // see shared_slots
     const int row0 = blockIdx.x / channel_blocks * ROWS;
     const int c = (blockIdx.x % channel_blocks * kConvThreads + threadIdx.x) * V;
     const int n = max(min(a.channels - c, V), 0);
-    long long slot[ROWS];
+    int slot[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int row = row0 + i;
@@ -281,27 +281,15 @@ conv_step_kernel(const SsdConvStepArgs a, int channel_blocks) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int in = slot[i] >= 0 ? n : 0;
-        const T* state = static_cast<const T*>(a.state) + (in ? slot[i] * a.state_stride + c : 0);
+        const T* state = static_cast<const T*>(a.state) + (in ? static_cast<long long>(slot[i]) * a.state_stride + c : 0);
 #pragma unroll
         for (int k = 0; k + 1 < W; ++k) load_raw<VECTOR, true>(raw[i][k], state + static_cast<long long>(k) * a.channels, in);
         load_raw<VECTOR, false>(raw[i][W - 1], static_cast<const T*>(a.x) + (in ? (row0 + i) * a.x_stride + c : 0), in);
     }
-    if (threadIdx.x == 0) flags = 0;
+    shared_slots<ROWS, kConvThreads>(slot, a.slots, a.rows, row0, flags);
     Filter<T, V, W> f;
     f.load(a.weight, a.bias, a.weight_f32, a.channels, c - threadIdx.x * V);
-    unsigned found = 0;
-    if (a.slots != nullptr) {
-        unsigned bits = 0;
-        for (int r = threadIdx.x; r < a.rows; r += kConvThreads) {
-            const int other = a.slots[r];
-#pragma unroll
-            for (int i = 0; i < ROWS; ++i)
-                if (other == slot[i] && r != row0 + i) bits |= r < row0 + i ? 1u << i : 0x10000u << i;
-        }
-        if (bits != 0) atomicOr(&flags, bits);
-        __syncthreads();
-        found = flags;
-    }
+    const unsigned found = a.slots != nullptr ? any_flag(flags) : 0;
     auto token = [&](const Pack<T, V> (&held)[W], int row) {
         float o[V];
 #pragma unroll
@@ -332,7 +320,7 @@ conv_step_kernel(const SsdConvStepArgs a, int channel_blocks) {
                     load_raw<VECTOR, false>(raw[i][W - 1], static_cast<const T*>(a.x) + r * a.x_stride + c, n);
                     token(raw[i], r);
                 }
-        T* next = static_cast<T*>(a.state_out) + slot[i] * a.state_out_stride + c;
+        T* next = static_cast<T*>(a.state_out) + static_cast<long long>(slot[i]) * a.state_out_stride + c;
 #pragma unroll
         for (int k = 1; k < W; ++k) store_raw<VECTOR>(next + static_cast<long long>(k - 1) * a.channels, raw[i][k], n);
     }

@@ -208,6 +208,30 @@ inline bool row_steps(S... elements) {
     return ((elements >= 0 && elements < (1 << 29)) && ...);
 }
 
+// ---- rows of a generation step that name the same slot.  Of a CTA's ROWS rows from row0 on: bit i, row i's slot is taken by an
+// earlier row; bit 16 + i, a later row names it too.  Every warp leaves what its threads found in flags[warp]; any_flag
+// joins them behind a barrier of the caller's.
+template <int ROWS, int THREADS>
+__device__ __forceinline__ void shared_slots(const int (&slot)[ROWS], const int* slots, int rows, int row0, unsigned* flags) {
+    if (slots == nullptr) return;
+    unsigned bits = 0;
+    for (int r = threadIdx.x; r < rows; r += THREADS) {
+        const int other = __ldg(slots + r);
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+            if (other == slot[i] && r != row0 + i) bits |= r < row0 + i ? 1u << i : 0x10000u << i;
+    }
+    bits = __reduce_or_sync(0xffffffffu, bits);
+    if ((threadIdx.x & 31) == 0) flags[threadIdx.x >> 5] = bits;
+}
+template <int WARPS>
+__device__ __forceinline__ unsigned any_flag(const unsigned (&flags)[WARPS]) {
+    unsigned bits = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) bits |= flags[w];
+    return bits;
+}
+
 // ---- sums over the rows of a table [rows][cols] in a fixed order: the second half of gradients of parameters.
 // Cell (r, c) of `out` gets the sum of column `col`; StoreCol(col, sum) writes it.
 constexpr int kSumCols = 32, kSumRows = 32;
