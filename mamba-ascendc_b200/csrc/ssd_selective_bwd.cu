@@ -226,7 +226,7 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
             F2 end_h = {}, end_g = {};
 #pragma unroll
             for (int i = 0; i < kTokens; ++i) {
-                al[i] = pack2(ex2f(dt[i].x * a2.x), ex2f(dt[i].y * a2.y));
+                al[i] = pack2(decay(dt[i].x, a2.x), decay(dt[i].y, a2.y));
                 h[i] = pack2(u[i].x * bt[i], u[i].y * bt[i]);
                 end_h = fma2(al[i], end_h, h[i]);
             }
@@ -234,7 +234,7 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
             for (int i = kTokens - 1; i >= 0; --i)
                 end_g = pack2(al[i].x * fmaf(ct[i], dy[i].x, end_g.x), al[i].y * fmaf(ct[i], dy[i].y, end_g.y));
             {
-                const float px = ex2f(sum_dt.x * a2.x), py = ex2f(sum_dt.y * a2.y);
+                const float px = decay(sum_dt.x, a2.x), py = decay(sum_dt.y, a2.y);
                 eh[w * 32] = make_float4(px, py, end_h.x, end_h.y);
                 eh[to_h_g + w * 32] = make_float4(px, py, end_g.x, end_g.y);
             }

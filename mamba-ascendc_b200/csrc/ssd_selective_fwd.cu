@@ -213,7 +213,7 @@ selective_walk_kernel(const SsdScanArgs a, const ScanLaunch l) {
 #pragma unroll
             for (int j = 0; j < NPL; ++j)
 #pragma unroll
-                for (int i = 0; i < kGroup; ++i) e[j][i] = ex2f(now.dt[i] * a2[j]);
+                for (int i = 0; i < kGroup; ++i) e[j][i] = decay(now.dt[i], a2[j]);
 #pragma unroll
             for (int group = 0; group < kGroups; ++group) {
                 if (group + kAhead < kGroups) fetch(kAhead == 2 ? third : next, group + kAhead);
@@ -236,7 +236,7 @@ selective_walk_kernel(const SsdScanArgs a, const ScanLaunch l) {
                     }
                     if (group + 1 < kGroups) {
 #pragma unroll
-                        for (int j = 0; j < NPL; ++j) e_next[j][t] = ex2f(next.dt[t] * a2[j]);
+                        for (int j = 0; j < NPL; ++j) e_next[j][t] = decay(next.dt[t], a2[j]);
                     }
                 }
                 if (kMode == kForward) {
@@ -324,7 +324,7 @@ selective_join_kernel(const SsdScanArgs a, const SeqMap map, float* work, const 
         float* at = work + item * per + static_cast<long long>(n) * a.channels + c;
         const float own = *at;
         *at = v;
-        v = fmaf(ex2f(a2 * sums[item * a.channels + c]), v, own);
+        v = fmaf(decay(sums[item * a.channels + c], a2), v, own);
     }
 }
 

@@ -113,7 +113,7 @@ selective_step_kernel(const SsdScanStepArgs a, const ScanBlocks b) {
             const float b4[4] = {bv.x, bv.y, bv.z, bv.w}, c4[4] = {cv.x, cv.y, cv.z, cv.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                s[j + k] = fmaf(ex2f(t.x * a2[j + k]), s[j + k], t.y * b4[k]);
+                s[j + k] = fmaf(decay(t.x, a2[j + k]), s[j + k], t.y * b4[k]);
                 y = fmaf(c4[k], s[j + k], y);
             }
         }
