@@ -65,6 +65,18 @@ __device__ __forceinline__ void unpack(float (&f)[V], const Pack<T, V>& raw) {
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = to_f(raw.v[i]);
 }
+// The same into shared memory without waiting, zeros if not `in`; a thread waits for its own copies.
+template <int V, class T>
+__device__ __forceinline__ void copy_async(Pack<T, V>& to, const T* p, bool in) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(&to))), "l"(p),
+                 "n"(sizeof(to)), "r"(in ? static_cast<int>(sizeof(to)) : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
 template <bool VECTOR, int V, class T>
 __device__ __forceinline__ void load_f(float (&f)[V], const T* p, int n) {
     Pack<T, V> raw;

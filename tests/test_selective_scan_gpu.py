@@ -517,3 +517,73 @@ def test_offsets_past_32_bits():
         arguments, options = step_inputs(tensors)
         one = ak.selective_scan_step(*arguments, cache, **options, slots=torch.tensor([slots - 1], dtype=torch.int32, device="cuda"))
         assert torch.equal(one, ak.selective_scan_step(*arguments, state, **options)) and torch.equal(cache[-1:], state)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,l,c,n,g,gated,skip", [
+    (1, 256, 64, 8, 1, True, True), (9, 257, 512, 8, 1, False, True), (2, 300, 64, 16, 2, True, False),
+    (9, 289, 512, 16, 1, False, False), (1, 290, 68, 32, 1, True, True), (1, 260, 36, 64, 1, True, True),
+    (1, 256, 32, 128, 1, True, False), (3, 273, 40, 12, 1, True, True),
+])
+def test_forward_of_long_sequences(b, l, c, n, g, gated, skip, dtype):
+    x, dt, A, B, C, D, z, bias, initial = make(b, l, c, n, g, dtype, seed=3)
+    D, z = D if skip else None, z if gated else None
+    out, final = ak.selective_scan(x, dt, A, B, C, D, z, bias, True, initial, return_final_state=True)
+    want, last = scan_plain(*map(double, (x, dt, A, B, C, D, z, bias)), True, double(initial))
+    top, top_h = magnitudes(x, dt, A, B, C, D, z, bias, True, initial)
+    near(out, want, top, rounding_count(l), "out", flush(l))
+    near(final, last, top_h, rounding_count(l), "final", flush(l))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_forward_of_long_packed_sequences(dtype):
+    lengths = [700, 0, 1, 33, 0, 1025, 290]
+    l, c, n = sum(lengths) + 7, 72, 16  # seven tokens behind the last sequence
+    x, dt, A, B, C, D, z, bias, initial = make(1, l, c, n, 2, dtype, states=len(lengths), seed=4)
+    edges = torch.tensor([0, *torch.tensor(lengths).cumsum(0).tolist()], dtype=torch.int32, device="cuda")
+    out, final = ak.selective_scan(x, dt, A, B, C, D, z, bias, True, initial, cu_seqlens=edges, return_final_state=True)
+    assert not out[:, l - 7:].any()
+    at = 0
+    for i, m in enumerate(lengths):
+        if m == 0:
+            assert torch.equal(final[i], initial[i])
+            continue
+        part = [None if t is None else t[:, at:at + m] for t in (x, dt, B, C, z)]
+        args = part[0], part[1], A, part[2], part[3], D, part[4], bias
+        want, last = scan_plain(*map(double, args), True, double(initial[i:i + 1]))
+        top, top_h = magnitudes(*args, True, initial[i:i + 1])
+        near(out[:, at:at + m], want, top, rounding_count(m), f"out {i}", flush(m))
+        near(final[i:i + 1], last, top_h, rounding_count(m), f"final {i}", flush(m))
+        at += m
+
+
+def test_long_segments_against_two_calls():
+    """A sequence of a few channels is cut into segments; the same one as two calls, joined by their states, is cut elsewhere.
+
+    All inputs are positive and dt is at least 0.05 with A at most -1, so that a term is below 2^-24 of its start after 340 tokens,
+    which bounds its roundings as at the top: 6 * 340 + 48 half steps of the value itself and one half step for what is behind, on
+    both sides.  Gradients of B and C add 64 channels, those of A the sums of 64 tokens and their joint sums."""
+    torch.manual_seed(5)
+    l, c, n = 40064, 64, 16
+    x, B, C, dout = (torch.rand(1, l, w, device="cuda") + 0.1 for w in (c, n, n, c))
+    dt = torch.rand(1, l, c, device="cuda") * 0.1 + 0.05
+    A = -(torch.rand(c, n, device="cuda") + 1)
+    start, dfinal = torch.rand(1, c, n, device="cuda"), torch.rand(1, c, n, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (x, A, B, C, start)]
+    x, A, B, C, start = leaves
+
+    def call(a, b, state):
+        return ak.selective_scan(x[:, a:b], dt[:, a:b], A, B[:, a:b, None], C[:, a:b, None], initial_states=state,
+                                 return_final_state=True)
+
+    out, final = call(0, l, start)
+    got = [out, final, *torch.autograd.grad([out, final], leaves, [dout, dfinal])]
+    half = 12000
+    first, state = call(0, half, start)
+    second, last = call(half, l, state)
+    both = torch.cat([first, second], 1)
+    want = [both, last, *torch.autograd.grad([both, last], leaves, [dout, dfinal])]
+    life = 6 * 340 + 50
+    for name, a, b, count in zip(("out", "final", "dx", "dA", "dB", "dC", "dinitial"), got, want,
+                                 (life, life, life, life + 64 + l // 64, life + 64, life + 64, life)):
+        near(a, b.double(), b.double().abs(), 2 * count, name, flush(l))
