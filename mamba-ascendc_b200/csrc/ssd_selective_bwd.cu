@@ -297,6 +297,17 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
             eh += n % 2 == 0 ? kWarps * 32 : -kWarps * 32;
             ea += n % 2 == 0 ? kWarps * 32 : -kWarps * 32;
         }
+        // on their way under the sums of the last column and the stores of dB and dC
+#pragma unroll
+        for (int i = 0; i < kTokens; ++i) {
+            const int t = tw + i, n = t < s.t1 ? pn : 0;
+            load_raw<VECTOR, false>(xr[i], xs.at(t), n);
+            load_raw<VECTOR, false>(dr[i], dts.at(t), n);
+            if (GATED) {
+                load_raw<VECTOR, false>(zr[i], zs.at(t), n);
+                load_raw<VECTOR, false>(gr[i], douts.at(t), n);
+            }
+        }
         __syncthreads();
         if (w == ((N - 1) & (kWarps - 1))) {
             float2 sum = dan[-32];
@@ -315,16 +326,6 @@ selective_bwd_kernel(const SsdScanGradArgs g, const BwdLaunch l) {
                     if (VECTOR || n + j < N) fb[j] = sb[(n + j) * kRow + quad_t], fc[j] = sc[(n + j) * kRow + quad_t];
                 store_f<VECTOR>(dbs.to(t0 + quad_t) + n, fb, min(N - n, 4));
                 store_f<VECTOR>(dcs.to(t0 + quad_t) + n, fc, min(N - n, 4));
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kTokens; ++i) {
-            const int t = tw + i, n = t < s.t1 ? pn : 0;
-            load_raw<VECTOR, false>(xr[i], xs.at(t), n);
-            load_raw<VECTOR, false>(dr[i], dts.at(t), n);
-            if (GATED) {
-                load_raw<VECTOR, false>(zr[i], zs.at(t), n);
-                load_raw<VECTOR, false>(gr[i], douts.at(t), n);
             }
         }
 #pragma unroll
