@@ -76,7 +76,8 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
     x [R,C]; ``slots`` int32 [R] says which slot of ``state`` a row takes (None: its own).  A number below zero or behind the
     last slot marks a row of padding, whose output is zeros; a slot that several rows name takes them one after another.
     ``state_out``, like ``state``: receives the new states instead, and slots that no row names are left as they were in
-    either.  Slots may lie apart, as one layer's share of a larger cache does.  Without gradients."""
+    either.  Slots may lie apart, as one layer's share of a larger cache does.  Without gradients; what is written counts as
+    changed in place for autograd."""
     if activation is None or activation == "silu":
         got = calls.short_conv_step(x, state, weight, bias, activation is not None, slots, state_out)
         if got is not None:
@@ -87,7 +88,7 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
         fail(op, "x must have shape [R,C]")
     _silu(op, activation)
     width = _check_filter(op, x, weight, bias)
-    without_gradients(op, x, state, weight, bias)
+    without_gradients(op, x, state, weight, bias, state_out)
     inner = (width - 1, x.shape[1])
     cache(op, state, "state", inner, x.dtype, x)
     if state_out is not None:

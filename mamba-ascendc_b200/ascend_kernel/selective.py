@@ -81,13 +81,13 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     row takes (None: its own).  A number below zero or behind the last slot marks a row of padding, whose output is zeros;
     a slot that several rows name takes them one after another.  ``state_out``, like ``state``: receives the new states
     instead, and slots that no row names are left as they were in either.  Slots may lie apart, as one layer's share of a
-    larger cache does.  Without gradients."""
+    larger cache does.  Without gradients; what is written counts as changed in place for autograd."""
     got = calls.selective_scan_step(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus, slots, state_out)
     if got is not None:
         return got
     op = "selective_scan_step"
     _check(op, 1, x, dt, A, B, C, D, z, dt_bias)
-    without_gradients(op, x, dt, A, B, C, D, z, dt_bias, state)
+    without_gradients(op, x, dt, A, B, C, D, z, dt_bias, state, state_out)
     inner = tuple(A.shape)
     cache(op, state, "state", inner, torch.float32, x)
     if state_out is not None:

@@ -143,6 +143,11 @@ bool slot_numbers(const Tensor& slots, const Tensor& x, const Tensor& state) {
     if (!slots.defined()) return state.size(0) == x.size(0);
     return slots.scalar_type() == at::kInt && whole(slots, {x.size(0)}, x);
 }
+// The slots are written through their pointer, so the framework is told that the tensor (and what it is a view of) changed: what
+// was saved of it for a backward pass is an error there.  Tensors of inference mode have no version and are never saved.
+void changed(const Tensor& state) {
+    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+}
 bool packing(const Tensor& cu, const Tensor& x) {
     return cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.numel() >= 2 && whole(cu, cu.sizes(), x) && x.size(0) == 1;
 }
@@ -402,7 +407,7 @@ std::optional<variable_list> short_conv_call(const Tensor& x, const Tensor& weig
 std::optional<variable_list> short_conv_step_call(const Tensor& x, const Tensor& state, const Tensor& weight, const Tensor& bias,
                                                   bool silu, const Tensor& slots, const Tensor& state_out) {
     if (!dense(x) || dtype_of(x) < 0 || x.dim() != 2 || !rowwise(x) || !filter_takes(x, weight, bias) ||
-        wants_grad(x, state, weight, bias))
+        wants_grad(x, state, weight, bias, state_out))
         return std::nullopt;
     const int64_t inner[2] = {weight.size(1) - 1, x.size(1)};
     const Tensor& next = state_out.defined() ? state_out : state;
@@ -431,6 +436,7 @@ std::optional<variable_list> short_conv_step_call(const Tensor& x, const Tensor&
     a.weight_f32 = f32(weight);
     a.silu = silu;
     check(lib.conv_step(&a, stream_of(x)), "short_conv_step");
+    changed(next);
     return variable_list{out};
 }
 
@@ -568,7 +574,8 @@ std::optional<variable_list> selective_scan_step_call(const Tensor& x, const Ten
                                                       const Tensor& C, const Tensor& state, const Tensor& D, const Tensor& z,
                                                       const Tensor& bias, bool softplus, const Tensor& slots,
                                                       const Tensor& state_out) {
-    if (!scan_takes(1, x, dt, A, B, C, D, z, bias) || wants_grad(x, dt, A, B, C, D, z, bias, state)) return std::nullopt;
+    if (!scan_takes(1, x, dt, A, B, C, D, z, bias) || wants_grad(x, dt, A, B, C, D, z, bias, state, state_out))
+        return std::nullopt;
     const int64_t inner[2] = {x.size(1), A.size(1)};
     const Tensor& next = state_out.defined() ? state_out : state;
     if (!cache(state, inner, at::kFloat, x) || !slot_numbers(slots, x, state)) return std::nullopt;
@@ -606,6 +613,7 @@ std::optional<variable_list> selective_scan_step_call(const Tensor& x, const Ten
     a.dtype = dtype_of(x);
     a.softplus = softplus;
     check(lib.scan_step(&a, stream_of(x)), "selective_scan_step");
+    changed(next);
     return variable_list{out};
 }
 
