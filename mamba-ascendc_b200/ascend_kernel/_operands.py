@@ -21,6 +21,16 @@ def unsupported(op: str) -> None:
     fail(op, "takes plain strided CUDA tensors only")
 
 
+def underived(op: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Neither inside a function transform nor with forward-mode derivatives, which the kernels would lose."""
+    tensors = [t for t in tensors if t is not None]
+    transforms, forward = torch._C._functorch, torch.autograd.forward_ad
+    if any(transforms.is_legacy_batchedtensor(t) or transforms.is_functorch_wrapped_tensor(t) for t in tensors):
+        fail(op, "cannot run inside a function transform (vmap, grad, jvp)")
+    if forward._current_level >= 0 and any(forward.unpack_dual(t).tangent is not None for t in tensors):
+        fail(op, "has no forward-mode derivatives")
+
+
 def activation(op: str, t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
     """A CUDA tensor of one of the activations' types, its columns side by side; ``like`` says which type and device."""
     if not t.is_cuda:

@@ -13,8 +13,8 @@ from typing import Optional, Tuple, Union
 import torch
 
 from ._capi import calls
-from ._operands import (activation as check_activation, cache, exactly, fail, packing, parameter, slot_numbers, unsupported,
-                        without_gradients)
+from ._operands import (activation as check_activation, cache, exactly, fail, packing, parameter, slot_numbers, underived,
+                        unsupported, without_gradients)
 
 
 def _silu(op: str, name: Optional[str]) -> None:
@@ -55,6 +55,7 @@ def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
         if got is not None:
             return got
     op = "short_conv"
+    underived(op, x, weight, bias, initial_states, cu_seqlens)
     check_activation(op, x, "x")
     if x.dim() != 3:
         fail(op, "x must have shape [B,L,C]")
@@ -83,6 +84,7 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
         if got is not None:
             return got
     op = "short_conv_step"
+    underived(op, x, state, weight, bias, slots, state_out)
     check_activation(op, x, "x")
     if x.dim() != 2:
         fail(op, "x must have shape [R,C]")

@@ -13,7 +13,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from ._capi import calls
-from ._operands import activation, exactly, fail, parameter, unsupported, without_gradients
+from ._operands import activation, exactly, fail, parameter, underived, unsupported, without_gradients
 
 MAX_WIDTH = 16384
 
@@ -46,6 +46,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     if got is not None:
         return got
     op = "rms_norm"
+    underived(op, x, weight, residual)
     _check(op, x, weight, residual)
     unsupported(op)
 
@@ -63,6 +64,7 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: Optional[tor
         if got is not None:
             return got
     op = "rms_norm_quant"
+    underived(op, x, weight, residual, scale)
     _check(op, x, weight, residual)
     without_gradients(op, x, weight, residual)
     if group_size is not None and (group_size not in (32, 64, 128) or x.shape[-1] % group_size):

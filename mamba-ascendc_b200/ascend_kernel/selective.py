@@ -15,7 +15,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from ._capi import calls
-from ._operands import activation, cache, fail, packing, parameter, slot_numbers, unsupported, without_gradients
+from ._operands import activation, cache, fail, packing, parameter, slot_numbers, underived, unsupported, without_gradients
 
 MAX_STATE = 128
 
@@ -64,6 +64,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     if got is not None:
         return got
     op = "selective_scan"
+    underived(op, x, dt, A, B, C, D, z, dt_bias, initial_states, cu_seqlens)
     _check(op, 2, x, dt, A, B, C, D, z, dt_bias)
     rows = x.shape[0] if cu_seqlens is None else packing(op, cu_seqlens, x)
     if initial_states is not None:
@@ -86,6 +87,7 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     if got is not None:
         return got
     op = "selective_scan_step"
+    underived(op, x, dt, A, B, C, state, D, z, dt_bias, slots, state_out)
     _check(op, 1, x, dt, A, B, C, D, z, dt_bias)
     without_gradients(op, x, dt, A, B, C, D, z, dt_bias, state, state_out)
     inner = tuple(A.shape)

@@ -75,7 +75,8 @@ int dtype_of(const Tensor& t) {
         default: return -1;
     }
 }
-bool dense(const Tensor& t) { return t.is_cuda() && t.layout() == at::kStrided; }
+// (inside a function transform a tensor has no storage of its own)
+bool dense(const Tensor& t) { return t.has_storage() && t.is_cuda() && t.layout() == at::kStrided; }
 // columns side by side
 bool rowwise(const Tensor& t) { return t.dim() > 0 && (t.stride(-1) == 1 || t.size(-1) <= 1); }
 bool activation(const Tensor& t, const Tensor& like) {
@@ -92,7 +93,11 @@ const Tensor& of(const Maybe& t) {
     static const Tensor none;
     return t.has_value() ? *t : none;
 }
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* ptr(const Tensor& t) {
+    // what a call allocates, and gradients that come in, can be tensors of a transform as well
+    TORCH_CHECK(!t.defined() || t.has_storage(), "ascend_kernel: cannot run inside a function transform (vmap, grad, jvp)");
+    return t.defined() ? t.data_ptr() : nullptr;
+}
 template <class T>
 T* ptr_as(const Tensor& t) { return static_cast<T*>(ptr(t)); }
 ssd_stream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
@@ -104,6 +109,14 @@ Tensor scratch(size_t bytes, const Tensor& like) {
 template <class... T>
 bool wants_grad(const T&... t) {
     return at::GradMode::is_enabled() && ((t.defined() && t.requires_grad()) || ...);
+}
+// Whether a forward-mode derivative is being taken with respect to one of them, which the kernels would lose.
+template <class... T>
+bool has_tangent(const T&... t) {
+    return ((t.defined() && t._fw_grad(/*level=*/0).defined()) || ...);
+}
+void check_upstream(const Tensor& dout, const Tensor& other, const char* op) {
+    TORCH_CHECK(!has_tangent(dout, other), op, ": its gradients have no forward-mode derivatives");
 }
 Tensor side_by_side(const Tensor& t) { return rowwise(t) ? t : t.contiguous(); }
 
@@ -234,6 +247,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
         const bool has_residual = types[1] != 0;
         Tensor dout = upstream[0], dstream = upstream.size() > 1 ? upstream[1] : Tensor();
         if (!dout.defined() && !dstream.defined()) return variable_list(4);
+        check_upstream(dout, dstream, "rms_norm");
         const c10::cuda::CUDAGuard guard(stream.device());
         const auto options = stream.options().dtype(x_type).requires_grad(false);
         dout = dout.defined() ? as_rows(side_by_side(dout)) : at::zeros(stream.sizes(), options);
@@ -274,7 +288,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
 };
 
 std::optional<variable_list> rms_norm_call(const Tensor& x, const Tensor& weight, const Tensor& residual, double eps) {
-    if (!norm_takes(x, weight, residual)) return std::nullopt;
+    if (!norm_takes(x, weight, residual) || has_tangent(x, weight, residual)) return std::nullopt;
     if (x.numel() == 0) {
         const Tensor stream = residual.defined() ? residual + x.to(residual.scalar_type()) : x;
         const Tensor out = stream.to(x.scalar_type()) * weight.to(x.scalar_type());
@@ -285,7 +299,9 @@ std::optional<variable_list> rms_norm_call(const Tensor& x, const Tensor& weight
 }
 std::optional<variable_list> rms_norm_quant_call(const Tensor& x_in, const Tensor& weight, const Tensor& residual_in, double eps,
                                                  int64_t group, const Tensor& scale) {
-    if (!norm_takes(x_in, weight, residual_in) || wants_grad(x_in, weight, residual_in)) return std::nullopt;
+    if (!norm_takes(x_in, weight, residual_in) || wants_grad(x_in, weight, residual_in) ||
+        has_tangent(x_in, weight, residual_in, scale))
+        return std::nullopt;
     const int64_t width = x_in.size(-1);
     if (group != 0 && ((group != 32 && group != 64 && group != 128) || width % group != 0)) return std::nullopt;
     if (scale.defined() && (group != 0 || !f32(scale) || scale.numel() != 1 || !whole(scale, scale.sizes(), x_in))) return std::nullopt;
@@ -361,6 +377,7 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
         const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &initial = saved[3], &cu = saved[4];
         Tensor dout = upstream[0], dfinal = upstream.size() > 1 ? upstream[1] : Tensor();
         if (!dout.defined() && !dfinal.defined()) return variable_list(7);
+        check_upstream(dout, dfinal, "short_conv");
         const c10::cuda::CUDAGuard guard(x.device());
         dout = dout.defined() ? dout.contiguous() : at::zeros(x.sizes(), x.options().requires_grad(false));
         if (dfinal.defined()) dfinal = dfinal.contiguous();
@@ -390,7 +407,9 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
 
 std::optional<variable_list> short_conv_call(const Tensor& x, const Tensor& weight, const Tensor& bias, bool silu,
                                              const Tensor& initial, const Tensor& cu, bool want_final) {
-    if (!dense(x) || dtype_of(x) < 0 || x.dim() != 3 || !rowwise(x) || !filter_takes(x, weight, bias)) return std::nullopt;
+    if (!dense(x) || dtype_of(x) < 0 || x.dim() != 3 || !rowwise(x) || !filter_takes(x, weight, bias) ||
+        has_tangent(x, weight, bias, initial))
+        return std::nullopt;
     if (cu.defined() && !packing(cu, x)) return std::nullopt;
     const int64_t rows = cu.defined() ? cu.numel() - 1 : x.size(0), channels = x.size(2), held = weight.size(1) - 1;
     if (initial.defined() && (initial.scalar_type() != x.scalar_type() || !whole(initial, {rows, held, channels}, x)))
@@ -407,7 +426,7 @@ std::optional<variable_list> short_conv_call(const Tensor& x, const Tensor& weig
 std::optional<variable_list> short_conv_step_call(const Tensor& x, const Tensor& state, const Tensor& weight, const Tensor& bias,
                                                   bool silu, const Tensor& slots, const Tensor& state_out) {
     if (!dense(x) || dtype_of(x) < 0 || x.dim() != 2 || !rowwise(x) || !filter_takes(x, weight, bias) ||
-        wants_grad(x, state, weight, bias, state_out))
+        wants_grad(x, state, weight, bias, state_out) || has_tangent(x, state, weight, bias, state_out))
         return std::nullopt;
     const int64_t inner[2] = {weight.size(1) - 1, x.size(1)};
     const Tensor& next = state_out.defined() ? state_out : state;
@@ -521,6 +540,7 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
         const Tensor &x = s[0], &A = s[2], &D = s[5], &z = s[6], &bias = s[7], &initial = s[8];
         Tensor dout = upstream[0], dfinal = upstream.size() > 1 ? upstream[1] : Tensor();
         if (!dout.defined() && !dfinal.defined()) return variable_list(12);
+        check_upstream(dout, dfinal, "selective_scan");
         const c10::cuda::CUDAGuard guard(x.device());
         dout = dout.defined() ? dout.contiguous() : at::zeros(x.sizes(), x.options().requires_grad(false));
         if (dfinal.defined()) dfinal = dfinal.contiguous();
@@ -557,7 +577,9 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
 std::optional<variable_list> selective_scan_call(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
                                                  const Tensor& D, const Tensor& z, const Tensor& bias, bool softplus,
                                                  const Tensor& initial, const Tensor& cu, bool want_final) {
-    if (!scan_takes(2, x, dt, A, B, C, D, z, bias) || (cu.defined() && !packing(cu, x))) return std::nullopt;
+    if (!scan_takes(2, x, dt, A, B, C, D, z, bias) || (cu.defined() && !packing(cu, x)) ||
+        has_tangent(x, dt, A, B, C, D, z, bias, initial))
+        return std::nullopt;
     const int64_t rows = cu.defined() ? cu.numel() - 1 : x.size(0), channels = x.size(2), n = A.size(1);
     if (initial.defined() && (!f32(initial) || !whole(initial, {rows, channels, n}, x))) return std::nullopt;
     if (x.numel() == 0 && (!cu.defined() || channels == 0)) {  // no tokens: the states pass through
@@ -574,7 +596,8 @@ std::optional<variable_list> selective_scan_step_call(const Tensor& x, const Ten
                                                       const Tensor& C, const Tensor& state, const Tensor& D, const Tensor& z,
                                                       const Tensor& bias, bool softplus, const Tensor& slots,
                                                       const Tensor& state_out) {
-    if (!scan_takes(1, x, dt, A, B, C, D, z, bias) || wants_grad(x, dt, A, B, C, D, z, bias, state, state_out))
+    if (!scan_takes(1, x, dt, A, B, C, D, z, bias) || wants_grad(x, dt, A, B, C, D, z, bias, state, state_out) ||
+        has_tangent(x, dt, A, B, C, D, z, bias, state, state_out))
         return std::nullopt;
     const int64_t inner[2] = {x.size(1), A.size(1)};
     const Tensor& next = state_out.defined() ? state_out : state;
