@@ -220,7 +220,7 @@ conv_bwd_kernel(const SsdConvGradArgs g, const ConvDims d, int slices) {
                 unpack(xs, xr[i]);
                 unpack(ds, dr[i]);
                 const int to = t + i - (W - 1);  // the input whose gradient is complete with this token
-                const bool mine = t + i < s.t1;
+                const bool mine = t + i < s.t1, there = t + i < end;
                 float o[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
@@ -233,8 +233,8 @@ conv_bwd_kernel(const SsdConvGradArgs g, const ConvDims d, int slices) {
 #pragma unroll
                         for (int k = 0; k < W; ++k) p = fmaf(f.w[k][j], held[k][j], p);
                         const float gate = sigmoid_fast(p);
-                        // behind the sequence's end there is no gradient, and inputs that are not there may make 0 * inf
-                        e = e == 0.f ? 0.f : e * gate * fmaf(p, 1.f - gate, 1.f);
+                        // behind the sequence's end there is no gradient, and what is still held of it may make 0 * inf
+                        e = there ? e * gate * fmaf(p, 1.f - gate, 1.f) : 0.f;
                     }
                     dpre[W - 1][j] = e;
                     if (mine) {

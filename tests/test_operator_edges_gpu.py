@@ -1,0 +1,56 @@
+"""Ends of the range that the documentation of the operators allows."""
+import pytest
+import torch
+
+import ascend_kernel as ak
+from operator_checks import conv_plain
+
+pytestmark = pytest.mark.gpu
+
+
+def rnd(*shape):
+    return torch.randn(*shape, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", [None, "silu"])
+def test_convolution_gradients_of_what_is_not_finite(act, dtype):
+    """Infinities and NaN in x, with upstream gradients of zero there and elsewhere: NaN where the definition has NaN (zero times
+    a derivative that is none) and nowhere else."""
+    b, l, c, w = 2, 40, 16, 4
+    x, weight, bias, initial = rnd(b, l, c).to(dtype), rnd(c, w), rnd(c), rnd(b, w - 1, c).to(dtype)
+    x[0, 7, 1], x[0, 21, 2], x[1, 39, 3], x[1, 0, 4], initial[0, 1, 5] = float("inf"), float("nan"), float("-inf"), float("inf"), float("nan")
+    dout = rnd(b, l, c).to(dtype)
+    dout[:, ::2] = 0
+    dout[:, 18:28] = 0
+
+    def gradients(call, *tensors):
+        leaves = [t.detach().requires_grad_(True) for t in tensors]
+        return torch.autograd.grad(call(*leaves), leaves, dout.to(leaves[0].dtype))
+
+    got = gradients(lambda x, w, b, s: ak.short_conv(x, w, b, act, s), x, weight, bias, initial)
+    want = gradients(lambda x, w, b, s: conv_plain(x, w, b, act, s)[0], *(t.double() for t in (x, weight, bias, initial)))
+    clean = gradients(lambda x, w, b, s: ak.short_conv(x, w, b, act, s),
+                      *(t.nan_to_num(0.25, 0.25, 0.25) for t in (x, weight, bias, initial)))
+    for name, g, v, k in zip(("dx", "dweight", "dbias", "dinitial"), got, want, clean):
+        assert torch.equal(g.isnan(), v.isnan()), name
+        assert v.isnan().any() or act is None, name
+    assert torch.equal(got[0][..., 6:], clean[0][..., 6:]) and torch.equal(got[1][6:], clean[1][6:])
+
+
+def test_convolution_gradients_stay_within_their_sequence():
+    """An infinity in the last inputs of a packed sequence, whose gradients end there."""
+    c, lengths = 16, [11, 1, 17, 24]
+    x, weight, bias, dout = rnd(1, sum(lengths) + 3, c), rnd(c, 4), rnd(c), rnd(1, sum(lengths) + 3, c)
+    cu = torch.tensor([0] + lengths).cumsum(0).to("cuda", torch.int32)
+    results = []
+    for spoil in (False, True):
+        leaf = x.clone()
+        if spoil:
+            leaf[:, 10], leaf[:, 11], leaf[:, 52] = float("inf"), float("nan"), float("inf")
+        leaf.requires_grad_(True)
+        results.append(torch.autograd.grad(ak.short_conv(leaf, weight, bias, "silu", cu_seqlens=cu), leaf, dout)[0])
+    good, bad = results
+    for own in (slice(0, 7), slice(12, 29), slice(29, 49), slice(53, 56)):
+        assert torch.equal(good[:, own], bad[:, own])
+    assert bad[:, 7:12].isnan().any(-1).all() and not bad[:, 53:].any()
