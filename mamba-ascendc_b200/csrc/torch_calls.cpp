@@ -140,6 +140,18 @@ struct Edges {
     bool wanted(bool present) { return present && ctx->needs_input_grad(next++); }
 };
 
+// A batch without tokens or rows, or without channels: nothing is launched and the states pass through.  (Packed sequences
+// without tokens are launched.)
+bool empty_call(const Tensor& x, const Tensor& cu) { return x.numel() == 0 && (!cu.defined() || x.size(-1) == 0); }
+// Its gradients: zeros for what the call takes beside the initial state, in their order, and that of the initial state.
+variable_list unmoved(Edges& edges, std::initializer_list<Tensor> taken, const Tensor& initial, const Tensor& dfinal) {
+    variable_list grads;
+    for (const Tensor& t : taken) grads.push_back(edges.wanted(t.defined()) ? at::zeros_like(t, at::MemoryFormat::Contiguous) : Tensor());
+    const bool want_initial = edges.wanted(initial.defined());
+    grads.push_back(!want_initial ? Tensor() : dfinal.defined() ? dfinal.clone() : at::zeros_like(initial));
+    return grads;
+}
+
 // ---- slots of a cache
 bool cache(const Tensor& state, at::IntArrayRef inner, at::ScalarType type, const Tensor& x) {
     if (!dense(state) || state.device() != x.device() || state.scalar_type() != type ||
@@ -361,7 +373,10 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
         if (want_final) final = empty({a.rows, a.width - 1, a.channels}, x);
         a.out = ptr(out);
         a.final_state = ptr(final);
-        check(lib.conv_fwd(&a, stream_of(x)), "short_conv");
+        if (!empty_call(x, cu))
+            check(lib.conv_fwd(&a, stream_of(x)), "short_conv");
+        else if (want_final)
+            initial.defined() ? final.copy_(initial) : final.zero_();
         return want_final ? variable_list{out, final} : variable_list{out};
     }
     // Keeps its inputs; backward forms the sum in front of the activation again.
@@ -381,6 +396,12 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
         const c10::cuda::CUDAGuard guard(x.device());
         dout = dout.defined() ? dout.contiguous() : at::zeros(x.sizes(), x.options().requires_grad(false));
         if (dfinal.defined()) dfinal = dfinal.contiguous();
+        if (empty_call(x, cu)) {
+            Edges edges{ctx};
+            variable_list grads = unmoved(edges, {x, weight, bias}, initial, dfinal);
+            grads.resize(7);
+            return once(upstream, std::move(grads));
+        }
         Edges edges{ctx};
         const bool want_x = edges.wanted(true), want_weight = edges.wanted(true), want_bias = edges.wanted(bias.defined());
         const bool want_initial = edges.wanted(initial.defined());
@@ -414,11 +435,6 @@ std::optional<variable_list> short_conv_call(const Tensor& x, const Tensor& weig
     const int64_t rows = cu.defined() ? cu.numel() - 1 : x.size(0), channels = x.size(2), held = weight.size(1) - 1;
     if (initial.defined() && (initial.scalar_type() != x.scalar_type() || !whole(initial, {rows, held, channels}, x)))
         return std::nullopt;
-    if (x.numel() == 0 && (!cu.defined() || channels == 0)) {  // no tokens: the states pass through
-        if (!want_final) return variable_list{x.clone()};
-        return variable_list{x.clone(), initial.defined() ? initial.clone()
-                                                          : at::zeros({rows, held, channels}, x.options().requires_grad(false))};
-    }
     if (wants_grad(x, weight, bias, initial)) return ConvNode::apply(x, weight, maybe(bias), maybe(initial), maybe(cu), silu, want_final);
     return ConvNode::call(x, weight, bias, initial, cu, silu, want_final);
 }
@@ -513,6 +529,10 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
         SsdScanArgs a = scan_args(x, dt, A, B, C, D, z, bias, initial, cu, softplus);
         Tensor out = empty(x.sizes(), x), final;
         if (want_final) final = empty_f32({a.rows, a.channels, a.dstate}, x);
+        if (empty_call(x, cu)) {
+            if (want_final) initial.defined() ? final.copy_(initial) : final.zero_();
+            return want_final ? variable_list{out, final} : variable_list{out};
+        }
         if (checkpoints != nullptr) {
             *checkpoints = empty_f32({static_cast<int64_t>(lib.scan_checkpoints(&a) / sizeof(float))}, x);
             a.checkpoints = ptr_as<float>(*checkpoints);
@@ -544,6 +564,12 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
         const c10::cuda::CUDAGuard guard(x.device());
         dout = dout.defined() ? dout.contiguous() : at::zeros(x.sizes(), x.options().requires_grad(false));
         if (dfinal.defined()) dfinal = dfinal.contiguous();
+        if (empty_call(x, s[9])) {
+            Edges edges{ctx};
+            variable_list grads = unmoved(edges, {x, s[1], A, s[3], s[4], D, z, bias}, initial, dfinal);
+            grads.resize(12);
+            return once(upstream, std::move(grads));
+        }
         SsdScanGradArgs g{};
         g.forward = scan_args(x, s[1], A, s[3], s[4], D, z, bias, initial, s[9], ctx->saved_data["softplus"].toBool());
         g.forward.checkpoints = ptr_as<float>(s[10]);
@@ -582,11 +608,6 @@ std::optional<variable_list> selective_scan_call(const Tensor& x, const Tensor& 
         return std::nullopt;
     const int64_t rows = cu.defined() ? cu.numel() - 1 : x.size(0), channels = x.size(2), n = A.size(1);
     if (initial.defined() && (!f32(initial) || !whole(initial, {rows, channels, n}, x))) return std::nullopt;
-    if (x.numel() == 0 && (!cu.defined() || channels == 0)) {  // no tokens: the states pass through
-        if (!want_final) return variable_list{x.clone()};
-        return variable_list{x.clone(), initial.defined() ? initial.clone()
-                                                          : at::zeros({rows, channels, n}, A.options().requires_grad(false))};
-    }
     if (wants_grad(x, dt, A, B, C, D, z, bias, initial))
         return ScanNode::apply(x, dt, A, B, C, maybe(D), maybe(z), maybe(bias), maybe(initial), maybe(cu), softplus, want_final);
     return ScanNode::call(x, dt, A, B, C, D, z, bias, initial, cu, softplus, want_final, nullptr);

@@ -54,3 +54,27 @@ def test_convolution_gradients_stay_within_their_sequence():
     for own in (slice(0, 7), slice(12, 29), slice(29, 49), slice(53, 56)):
         assert torch.equal(good[:, own], bad[:, own])
     assert bad[:, 7:12].isnan().any(-1).all() and not bad[:, 53:].any()
+
+
+@pytest.mark.parametrize("b,l", [(2, 0), (0, 5), (0, 0)])
+def test_gradients_of_calls_without_tokens(b, l):
+    """Every tensor has its gradient: zeros for what nothing depends on, the states' own for what passes through."""
+    c, w, n = 16, 4, 8
+    x, weight, bias, initial = (t.requires_grad_(True) for t in (rnd(b, l, c), rnd(c, w), rnd(c), rnd(b, w - 1, c)))
+    out, final = ak.short_conv(x, weight, bias, "silu", initial, return_final_state=True)
+    grads = torch.autograd.grad([out, final], [x, weight, bias, initial], [torch.ones_like(out), 2 * torch.ones_like(final)])
+    assert [g.shape for g in grads] == [t.shape for t in (x, weight, bias, initial)]
+    assert not grads[1].any() and not grads[2].any() and (grads[3] == 2).all() and torch.equal(final, initial)
+    assert not torch.autograd.grad(ak.short_conv(x, weight).sum(), weight)[0].any()
+    alone = ak.short_conv(x.detach(), weight, None, None, return_final_state=True)[1]
+    assert not torch.autograd.grad(alone.sum(), weight)[0].any() and not alone.any()
+
+    tensors = [rnd(b, l, c), rnd(b, l, c), -rnd(c, n).abs(), rnd(b, l, 1, n), rnd(b, l, 1, n), rnd(c), rnd(b, l, c), rnd(c), rnd(b, c, n)]
+    for t in tensors:
+        t.requires_grad_(True)
+    out, final = ak.selective_scan(*tensors[:8], True, tensors[8], return_final_state=True)
+    grads = torch.autograd.grad([out, final], tensors, [torch.ones_like(out), 2 * torch.ones_like(final)])
+    assert [g.shape for g in grads] == [t.shape for t in tensors]
+    assert not any(g.any() for g in grads[:8]) and (grads[8] == 2).all() and torch.equal(final, tensors[8])
+    out, final = ak.selective_scan(*tensors[:5], return_final_state=True)
+    assert not final.any() and not torch.autograd.grad(out.sum() + final.sum(), tensors[2])[0].any()
