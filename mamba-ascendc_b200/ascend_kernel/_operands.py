@@ -102,6 +102,24 @@ def cache(op: str, state: torch.Tensor, name: str, inner: Tuple[int, ...], dtype
         fail(op, f"{name} must have its slots apart")
 
 
+def apart(op: str, state: torch.Tensor, state_out: torch.Tensor) -> None:
+    """Slot i of state_out may be slot i of state, and shares no memory with any other."""
+    count, size = state.shape[0], state.element_size()
+    inner = state[0].numel() * size if count else 0
+    if inner == 0:
+        return
+    step, step_out = (t.stride(0) * size if count > 1 else inner for t in (state, state_out))
+    distance = state_out.data_ptr() - state.data_ptr()
+    if distance >= (count - 1) * step + inner or -distance >= (count - 1) * step_out + inner:
+        return
+    for i in range(count):
+        at = distance + i * step_out
+        k = max(at, 0) // step
+        for near in range(k, min(k + 2, count)):
+            if at < near * step + inner and near * step < at + inner and not (near == i and at == i * step):
+                fail(op, "state_out must be state or lie apart from it")
+
+
 def without_gradients(op: str, *tensors: Optional[torch.Tensor]) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         fail(op, "has no gradients; call it under torch.no_grad()")

@@ -13,8 +13,8 @@ from typing import Optional, Tuple, Union
 import torch
 
 from ._capi import calls
-from ._operands import (activation as check_activation, cache, exactly, fail, packing, parameter, slot_numbers, underived,
-                        unsupported, without_gradients)
+from ._operands import (activation as check_activation, apart, cache, exactly, fail, packing, parameter, slot_numbers,
+                        underived, unsupported, without_gradients)
 
 
 def _silu(op: str, name: Optional[str]) -> None:
@@ -77,8 +77,8 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
     x [R,C]; ``slots`` int32 [R] says which slot of ``state`` a row takes (None: its own).  A number below zero or behind the
     last slot marks a row of padding, whose output is zeros; a slot that several rows name takes them one after another.
     ``state_out``, like ``state``: receives the new states instead, and slots that no row names are left as they were in
-    either.  Slots may lie apart, as one layer's share of a larger cache does.  Without gradients; what is written counts as
-    changed in place for autograd."""
+    either; it may be ``state``, but no slot of it may lie on another one of ``state``.  Slots may lie apart, as one layer's
+    share of a larger cache does.  Without gradients; what is written counts as changed in place for autograd."""
     if activation is None or activation == "silu":
         got = calls.short_conv_step(x, state, weight, bias, activation is not None, slots, state_out)
         if got is not None:
@@ -97,5 +97,6 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
         cache(op, state_out, "state_out", inner, x.dtype, x)
         if state_out.shape != state.shape:
             fail(op, "state_out must have the shape of state")
+        apart(op, state, state_out)
     slot_numbers(op, slots, x, state)
     unsupported(op)

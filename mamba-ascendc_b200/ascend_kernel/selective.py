@@ -15,7 +15,8 @@ from typing import Optional, Tuple, Union
 import torch
 
 from ._capi import calls
-from ._operands import activation, cache, fail, packing, parameter, slot_numbers, underived, unsupported, without_gradients
+from ._operands import (activation, apart, cache, fail, packing, parameter, slot_numbers, underived, unsupported,
+                        without_gradients)
 
 MAX_STATE = 128
 
@@ -81,7 +82,8 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     x, dt and z [R,C], B and C [R,G,N] as in ``selective_scan``; state fp32.  ``slots`` int32 [R] says which slot of ``state`` a
     row takes (None: its own).  A number below zero or behind the last slot marks a row of padding, whose output is zeros;
     a slot that several rows name takes them one after another.  ``state_out``, like ``state``: receives the new states
-    instead, and slots that no row names are left as they were in either.  Slots may lie apart, as one layer's share of a
+    instead, and slots that no row names are left as they were in either; it may be ``state``, but no slot of it may lie on
+    another one of ``state``.  Slots may lie apart, as one layer's share of a
     larger cache does.  Without gradients; what is written counts as changed in place for autograd."""
     got = calls.selective_scan_step(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus, slots, state_out)
     if got is not None:
@@ -96,5 +98,6 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
         cache(op, state_out, "state_out", inner, torch.float32, x)
         if state_out.shape != state.shape:
             fail(op, "state_out must have the shape of state")
+        apart(op, state, state_out)
     slot_numbers(op, slots, x, state)
     unsupported(op)

@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <optional>
 #include <string>
 
@@ -167,6 +168,27 @@ bool cache(const Tensor& state, at::IntArrayRef inner, at::ScalarType type, cons
 bool slot_numbers(const Tensor& slots, const Tensor& x, const Tensor& state) {
     if (!slots.defined()) return state.size(0) == x.size(0);
     return slots.scalar_type() == at::kInt && whole(slots, {x.size(0)}, x);
+}
+// Rows run at the same time, so a row's new state must not lie on what another row (or the row itself, elsewhere) reads: slot i of
+// `out` may share memory with slot i of `state` if they are the same, and with no other.
+bool apart(const Tensor& state, const Tensor& out) {
+    const int64_t count = state.size(0), bytes = state.element_size();
+    const int64_t inner = count > 0 ? state.numel() / count * bytes : 0;
+    if (inner == 0) return true;
+    const int64_t step = count > 1 ? state.stride(0) * bytes : inner, step_out = count > 1 ? out.stride(0) * bytes : inner;
+    const int64_t first = reinterpret_cast<intptr_t>(state.data_ptr()), first_out = reinterpret_cast<intptr_t>(out.data_ptr());
+    if (first + (count - 1) * step + inner <= first_out || first_out + (count - 1) * step_out + inner <= first) return true;
+    const int64_t distance = first_out - first;
+    if (step == step_out) {  // from each slot the same way to the next ones of the other
+        const int64_t rest = (distance % step + step) % step;
+        return distance == 0 || (rest >= inner && step - rest >= inner);
+    }
+    for (int64_t i = 0; i < count; ++i) {
+        const int64_t at = distance + i * step_out, k = at < 0 ? 0 : at / step;  // slot i of out lies at or behind slot k
+        for (int64_t near = k; near < std::min(k + 2, count); ++near)
+            if (at < near * step + inner && near * step < at + inner && !(near == i && at == i * step)) return false;
+    }
+    return true;
 }
 // The slots are written through their pointer, so the framework is told that the tensor (and what it is a view of) changed: what
 // was saved of it for a backward pass is an error there.  Tensors of inference mode have no version and are never saved.
@@ -447,7 +469,8 @@ std::optional<variable_list> short_conv_step_call(const Tensor& x, const Tensor&
     const int64_t inner[2] = {weight.size(1) - 1, x.size(1)};
     const Tensor& next = state_out.defined() ? state_out : state;
     if (!cache(state, inner, x.scalar_type(), x) || !slot_numbers(slots, x, state)) return std::nullopt;
-    if (state_out.defined() && (!cache(state_out, inner, x.scalar_type(), x) || state_out.size(0) != state.size(0)))
+    if (state_out.defined() &&
+        (!cache(state_out, inner, x.scalar_type(), x) || state_out.size(0) != state.size(0) || !apart(state, state_out)))
         return std::nullopt;
     const c10::cuda::CUDAGuard guard(x.device());
     if (x.numel() == 0 || state.size(0) == 0) return variable_list{at::zeros(x.sizes(), x.options().requires_grad(false))};
@@ -623,7 +646,9 @@ std::optional<variable_list> selective_scan_step_call(const Tensor& x, const Ten
     const int64_t inner[2] = {x.size(1), A.size(1)};
     const Tensor& next = state_out.defined() ? state_out : state;
     if (!cache(state, inner, at::kFloat, x) || !slot_numbers(slots, x, state)) return std::nullopt;
-    if (state_out.defined() && (!cache(state_out, inner, at::kFloat, x) || state_out.size(0) != state.size(0))) return std::nullopt;
+    if (state_out.defined() &&
+        (!cache(state_out, inner, at::kFloat, x) || state_out.size(0) != state.size(0) || !apart(state, state_out)))
+        return std::nullopt;
     const c10::cuda::CUDAGuard guard(x.device());
     if (x.numel() == 0 || state.size(0) == 0) return variable_list{at::zeros(x.sizes(), x.options().requires_grad(false))};
     const Tensor out = empty(x.sizes(), x);

@@ -4,6 +4,7 @@ import torch
 
 import ascend_kernel as ak
 from operator_checks import conv_plain
+from test_operator_overlap_cpu import hazard, small_views
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +79,56 @@ def test_gradients_of_calls_without_tokens(b, l):
     assert not any(g.any() for g in grads[:8]) and (grads[8] == 2).all() and torch.equal(final, tensors[8])
     out, final = ak.selective_scan(*tensors[:5], return_final_state=True)
     assert not final.any() and not torch.autograd.grad(out.sum() + final.sum(), tensors[2])[0].any()
+
+
+def overlapping(pool):
+    """(state, state_out) that share memory but are not the same slots."""
+    n, inner = pool.shape[0], pool[0].numel()
+    flat = pool.view(n, inner)
+    shifted = torch.as_strided(flat, pool[1:].shape, pool.stride(), inner // 2)
+    return [(pool[:-1], pool[1:]), (pool[1:], pool[:-1]), (pool[:-1], shifted), (pool[:2], pool[1:4:2])]
+
+
+def apart(pool):
+    """(state, state_out) that lie in one cache side by side, or are the same."""
+    n = pool.shape[0]
+    return [(pool, pool), (pool[::2], pool[1::2]), (pool[1::2], pool[::2]), (pool[:n // 2], pool[n // 2:]), (pool[::2], pool[::2]),
+            (pool[:4:2], pool[:2])]
+
+
+def test_state_out_that_overlaps_the_state_in_part():
+    """Rows run at the same time, so that one's new state would be another's old one or not, by chance."""
+    c, w, n = 8, 4, 16
+    for state, out in overlapping(rnd(6, w - 1, c)):
+        with pytest.raises(RuntimeError, match="short_conv_step: state_out must be state or lie apart from it"):
+            ak.short_conv_step(rnd(state.shape[0], c), state, rnd(c, w), state_out=out)
+    for state, out in apart(rnd(6, w - 1, c)):
+        x, weight, fresh = rnd(state.shape[0], c), rnd(c, w), torch.zeros_like(state)
+        want = ak.short_conv_step(x, state, weight, state_out=fresh)
+        assert torch.equal(ak.short_conv_step(x, state, weight, state_out=out), want) and torch.equal(out, fresh)
+
+    def arguments(r):
+        return rnd(r, c), rnd(r, c), -rnd(c, n).abs(), rnd(r, 1, n), rnd(r, 1, n)
+
+    for state, out in overlapping(rnd(6, c, n)):
+        with pytest.raises(RuntimeError, match="selective_scan_step: state_out must be state or lie apart from it"):
+            ak.selective_scan_step(*arguments(state.shape[0]), state, state_out=out)
+    for state, out in apart(rnd(6, c, n)):
+        a, fresh = arguments(state.shape[0]), torch.zeros_like(state)
+        want = ak.selective_scan_step(*a, state, state_out=fresh)
+        assert torch.equal(ak.selective_scan_step(*a, state, state_out=out), want) and torch.equal(out, fresh)
+
+
+def test_every_pair_of_views_of_a_small_cache():
+    """What is refused is refused before any launch; the rest gives what separate caches give."""
+    weight = rnd(1, 4)
+    for state, out in small_views(torch.randn(60, device="cuda")):
+        rows = state.shape[0]
+        state, out, x = state.view(rows, 3, 1), out.view(rows, 3, 1), rnd(rows, 1)
+        if hazard(state, out):
+            with pytest.raises(RuntimeError, match="state_out must be state or lie apart from it"):
+                ak.short_conv_step(x, state, weight, state_out=out)
+        else:
+            fresh = torch.empty(rows, 3, 1, device="cuda")
+            want = ak.short_conv_step(x, state.clone(), weight, state_out=fresh)
+            assert torch.equal(ak.short_conv_step(x, state, weight, state_out=out), want) and torch.equal(out, fresh)
