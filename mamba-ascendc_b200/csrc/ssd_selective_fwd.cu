@@ -498,14 +498,15 @@ ScanSegments scan_segments(const SsdScanArgs& a, int per_cta, int slots) {
     const ScanBlocks b = scan_blocks(a.channels, a.groups, per_cta);
     const long long ctas = static_cast<long long>(a.rows) * b.count(a.groups);
     const long long total = a.cu_seqlens ? a.tokens : a.tokens * a.rows;
-    ScanSegments s{1 << 30, 0, false};
+    constexpr int kWhole = 0x7fffffff;  // more than any sequence has
+    ScanSegments s{kWhole, 0, false};
     if (ctas * 2 < slots && total > 2 * kScanCheckpoint) {
         const long long span = total * b.count(a.groups) / (2LL * slots);
         s.span = static_cast<int>(span < kScanCheckpoint ? kScanCheckpoint
                                                          : (span + kScanCheckpoint - 1) / kScanCheckpoint * kScanCheckpoint);
         s.split = s.span < a.tokens;
     }
-    if (!s.split) s.span = 1 << 30;
+    if (!s.split) s.span = kWhole;
     s.items = scan_map(a, s.span).items();
     return s;
 }
