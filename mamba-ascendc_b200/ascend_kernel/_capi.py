@@ -203,4 +203,13 @@ def _load_calls():
     return module
 
 
-calls = _load_calls()
+class _Calls:
+    """The operators' calls; the module is loaded by the first of them, as the SSD does without it."""
+
+    def __getattr__(self, name: str):
+        module = _load_calls()
+        self.__dict__.update((n, f) for n, f in vars(module).items() if not n.startswith("_"))
+        return getattr(module, name)
+
+
+calls = _Calls()
