@@ -189,7 +189,7 @@ extern "C" const char* ssd_error_string(int code) {
                    "on the current device)";
         case SSD_ERR_RANGE:
             return "ssd: size out of range (batch and ngroups at most 65535; batch * seqlen and the number of state rows "
-                   "below 2^31)";
+                   "below 2^31; the operators' rows, tokens and slots below 2^31 and rows less than 2^31 bytes apart)";
         case SSD_ERR_ALIGN: return "ssd: tensor base addresses must be 16-byte aligned";
         case SSD_ERR_TENSORMAP: return "ssd: the CUDA driver rejected a TMA tensor map";
         case SSD_ERR_LAUNCH: return "ssd: kernel launch failed";

@@ -13,6 +13,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
+#include <limits>
 #include <optional>
 #include <string>
 
@@ -65,6 +66,12 @@ void bind(const py::dict& addresses) {
 
 void check(int code, const char* op) {
     TORCH_CHECK(code == SSD_OK, op, ": ", lib.error_string(code), " (code ", code, ")");
+}
+
+// A size as the records have it.
+int32_t number(int64_t size, const char* op) {
+    check(size <= std::numeric_limits<int32_t>::max() ? SSD_OK : SSD_ERR_RANGE, op);
+    return static_cast<int32_t>(size);
 }
 
 // ---- what a tensor is
@@ -377,8 +384,8 @@ SsdConvArgs conv_args(const Tensor& x, const Tensor& weight, const Tensor& bias,
     a.tokens = x.size(1);
     a.batch_stride = x.stride(0);
     a.token_stride = x.stride(1);
-    a.rows = static_cast<int32_t>(cu.defined() ? cu.numel() - 1 : x.size(0));
-    a.channels = static_cast<int32_t>(x.size(2));
+    a.rows = number(cu.defined() ? cu.numel() - 1 : x.size(0), "short_conv");
+    a.channels = number(x.size(2), "short_conv");
     a.width = static_cast<int32_t>(weight.size(1));
     a.dtype = dtype_of(x);
     a.weight_f32 = f32(weight);
@@ -486,9 +493,9 @@ std::optional<variable_list> short_conv_step_call(const Tensor& x, const Tensor&
     a.x_stride = x.stride(0);
     a.state_stride = state.stride(0);
     a.state_out_stride = next.stride(0);
-    a.rows = static_cast<int32_t>(x.size(0));
-    a.slot_count = static_cast<int32_t>(state.size(0));
-    a.channels = static_cast<int32_t>(x.size(1));
+    a.rows = number(x.size(0), "short_conv_step");
+    a.slot_count = number(state.size(0), "short_conv_step");
+    a.channels = number(x.size(1), "short_conv_step");
     a.width = static_cast<int32_t>(weight.size(1));
     a.dtype = dtype_of(x);
     a.weight_f32 = f32(weight);
@@ -535,10 +542,10 @@ SsdScanArgs scan_args(const Tensor& x, const Tensor& dt, const Tensor& A, const 
         a.b_strides[d] = B.stride(d);
         a.c_strides[d] = C.stride(d);
     }
-    a.rows = static_cast<int32_t>(cu.defined() ? cu.numel() - 1 : x.size(0));
-    a.channels = static_cast<int32_t>(x.size(2));
+    a.rows = number(cu.defined() ? cu.numel() - 1 : x.size(0), "selective_scan");
+    a.channels = number(x.size(2), "selective_scan");
     a.dstate = static_cast<int32_t>(A.size(1));
-    a.groups = static_cast<int32_t>(B.size(2));
+    a.groups = number(B.size(2), "selective_scan");
     a.dtype = dtype_of(x);
     a.softplus = softplus;
     return a;
@@ -674,11 +681,11 @@ std::optional<variable_list> selective_scan_step_call(const Tensor& x, const Ten
     }
     a.state_stride = state.stride(0);
     a.state_out_stride = next.stride(0);
-    a.rows = static_cast<int32_t>(x.size(0));
-    a.slot_count = static_cast<int32_t>(state.size(0));
-    a.channels = static_cast<int32_t>(x.size(1));
+    a.rows = number(x.size(0), "selective_scan_step");
+    a.slot_count = number(state.size(0), "selective_scan_step");
+    a.channels = number(x.size(1), "selective_scan_step");
     a.dstate = static_cast<int32_t>(A.size(1));
-    a.groups = static_cast<int32_t>(B.size(1));
+    a.groups = number(B.size(1), "selective_scan_step");
     a.dtype = dtype_of(x);
     a.softplus = softplus;
     check(lib.scan_step(&a, stream_of(x)), "selective_scan_step");

@@ -132,3 +132,18 @@ def test_every_pair_of_views_of_a_small_cache():
             fresh = torch.empty(rows, 3, 1, device="cuda")
             want = ak.short_conv_step(x, state.clone(), weight, state_out=fresh)
             assert torch.equal(ak.short_conv_step(x, state, weight, state_out=out), want) and torch.equal(out, fresh)
+
+
+def test_sizes_that_the_records_cannot_hold():
+    """2^32 + 5 rows (all at one place): as a 32-bit number they would be five."""
+    rows, c, n = 2 ** 32 + 5, 1, 1
+    x, weight = torch.zeros(1, 1, c, device="cuda", dtype=torch.bfloat16).expand(rows, 1, c), rnd(c, 4)
+    B, A = x.unsqueeze(2), -torch.ones(c, n, device="cuda")
+    slots = torch.zeros(1, device="cuda", dtype=torch.int32)
+    with torch.no_grad():
+        for call in (lambda: ak.short_conv(x, weight), lambda: ak.selective_scan(x, x, A, B, B)):
+            with pytest.raises(RuntimeError, match="out of range"):
+                call()
+        cache = torch.empty(rows, 1, c, device="cuda", dtype=torch.bfloat16)  # more slots than there are numbers for them
+        with pytest.raises(RuntimeError, match="short_conv_step: .*out of range"):
+            ak.short_conv_step(x[:1, 0], cache, rnd(c, 2), slots=slots)
