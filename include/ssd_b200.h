@@ -360,8 +360,9 @@ int ssd_short_conv_bwd(const SsdConvGradArgs* args, ssd_stream_t stream);
 
 /* One token of each of `rows` sequences: x [rows, channels] with rows x_stride apart, states [slots, width - 1, channels] with slots
  * state_stride (state_out_stride) apart.  Row r takes slot slots[r] (r itself where slots is null): its state is read from
- * `state`, and the one with the token is written to `state_out`, which may be `state`.  A slot below zero or behind the last is none: the row's
- * output is zeros.  A slot that several rows name takes them one after another, in their order. */
+ * `state`, and the one with the token is written to `state_out`, which may be `state`; none of its slots may lie on another
+ * one of `state`.  A slot below zero or behind the last is none: the row's output is zeros.  A slot that several rows name
+ * takes them one after another, in their order. */
 typedef struct SsdConvStepArgs {
     const void *x, *weight, *bias, *state;
     const int32_t* slots;

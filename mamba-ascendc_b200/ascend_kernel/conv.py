@@ -3,8 +3,9 @@ sequences, with the state that a later call goes on from) and for generation ste
 
     pre[t] = bias + sum_k weight[:, k] * in[t - (width - 1) + k] ;  out = pre, or pre * sigmoid(pre)
 
-The depthwise conv1d of every Mamba block (mamba_torch/vmamba2_network.py:197-302), token-major like the SSD's own tensors
-(``ssd_short_conv_fwd``, ``ssd_short_conv_bwd``, ``ssd_short_conv_step``).
+The depthwise conv1d of a Mamba block, token-major like the SSD's own tensors (``ssd_short_conv_fwd``, ``ssd_short_conv_bwd``,
+``ssd_short_conv_step``).  The reference has no such operator; its demo network has the framework's 3x3 convolution over the
+image in that place (mamba_torch/vmamba2_network.py:197-302).
 """
 from __future__ import annotations
 

@@ -2,9 +2,9 @@
 
     stream = x + residual ;  out = stream / sqrt(mean(stream^2) + eps) * weight
 
-The norm in front of every block of a Mamba network (mamba_torch/vmamba2_network.py:197-302 applies it with framework
-calls); one pass over the data each way (``ssd_rms_norm_fwd``, ``ssd_rms_norm_bwd``).  Rows are normed in fp32, before the
-sum is rounded to the residual's type.
+The norm in front of every block of a Mamba network; one pass over the data each way (``ssd_rms_norm_fwd``,
+``ssd_rms_norm_bwd``).  Rows are normed in fp32, before the sum is rounded to the residual's type.  The reference has no such
+operator; its demo network has the framework's layer norm in that place (mamba_torch/vmamba2_network.py:197-302).
 """
 from __future__ import annotations
 

@@ -8,8 +8,8 @@ namespace ssd {
 constexpr int kScanMaxState = 128;
 constexpr int kScanCheckpoint = 64;  // tokens between the states that backward starts from
 
-// Two fp32 values side by side.  (The packed fp32 instructions take two cycles each: with them the forward pass takes 559 us where
-// it takes 483 without, as they tie registers in pairs.)
+// Two fp32 values side by side.  (The packed fp32 instructions take two cycles each, so they save nothing, and tie registers in
+// pairs: the forward pass before its staging warps took 559 us with them and 483 without.)
 struct alignas(8) F2 {
     float x, y;
 };

@@ -3,8 +3,8 @@
 //   g_t = C_t dy_t + a_{t+1} g_{t+1} ;  dC_t[n] = sum_c dy_t h_t[n] ;  dB_t[n] = sum_c g_t[n] dt_t x_t ;  du_t = sum_n g_t[n] B_t[n]
 //   q_t[n] = g_t[n] a_t[n] h_{t-1}[n] ;  ddt_t = x_t du_t + sum_n q_t[n] A[n] ;  dA[n] = sum_t q_t[n] dt_t ;  dx_t = dt_t du_t + D dy_t
 //
-// What bounds it: instructions, 16 for the arithmetic of each (token, channel, state column) and about ten more: the sums of
-// dB and dC over the channels, which lie along the lanes, the exchange between the warps of a chunk, and what each (token,
+// What bounds it: instructions, 35 for each (token, channel, state column) as counted: 16 are the arithmetic, the others the sums
+// of dB and dC over the channels, which lie along the lanes, the exchange between the warps of a chunk, and what each (token,
 // channel) takes.  The bytes are few beside that.
 //
 // Layout: a lane owns two neighbouring channels, a warp kTokens tokens of 64 channels, a CTA a chunk of kWarps * kTokens tokens,

@@ -435,7 +435,8 @@ selective_join_kernel(const SsdScanArgs a, const SeqMap map, float* work, const 
 // columns per warp then, although each warp reads dt and dt x again (368 against 420 us for [1,8192,4096] with 16 columns).
 // With helpers, against without (us):   16 columns  [1,8192,4096] 297 / 364   [4,2000,2048] 129 / 142   [1,16384,1536] 316 / 402
 //   8 columns [1,8192,4096] 241 / 325   32 columns [1,8192,4096] 471 / 536   64 columns [1,4096,4096] 417 / 478.
-// With 128 columns the two tiles and the ring would not fit.
+// With 128 columns there are none: in fp32 the two tiles and the ring would take 287 KB, and in 16 bits, where they take 219, sixteen
+// warps leave a thread 128 registers, in which the forward walk spills 164 bytes (255 registers without staging warps).
 template <class F>
 int with_columns(int dstate, bool few, bool help, F f) {
     const auto is = [&](auto npl, auto nw) { return help ? f(npl, nw, std::true_type{}) : f(npl, nw, std::false_type{}); };
