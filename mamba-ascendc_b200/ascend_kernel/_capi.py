@@ -207,6 +207,8 @@ class _Calls:
     """The operators' calls; the module is loaded by the first of them, as the SSD does without it."""
 
     def __getattr__(self, name: str):
+        if name.startswith("_"):
+            raise AttributeError(name)
         module = _load_calls()
         self.__dict__.update((n, f) for n, f in vars(module).items() if not n.startswith("_"))
         return getattr(module, name)
